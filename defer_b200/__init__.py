@@ -11,6 +11,7 @@ C ABI in include/defer_b200.h:
     seed_from_u64, words_per_sample, sample_logits      (src/engine.rs, src/sampler.rs)
     DeferCheckpoint, WalHeader, WalWriter, WalLog       (src/checkpoint.rs, src/wal.rs)
     ablation_attribution, log_softmax_at                (src/attribution.rs)
+    Q8Cache, q8_append, q8_read, q8_attend              (no counterpart: a key/value cache in 8 bits)
 
 plus the batched drivers (replay_batch, generate_batch) that advance many
 sessions per device step. Every call runs the CUDA path; there is no CPU
@@ -25,8 +26,9 @@ from typing import Callable, List, Optional, Sequence
 
 import numpy as np
 
-from . import _lib
+from . import _lib, q8
 from ._lib import CheckpointFields, DeferConfig, TOKEN_CB, WalHeaderC
+from .q8 import Q8Cache, q8_append, q8_attend, q8_read
 
 __all__ = [
     "DeferError", "IoError", "ParseError", "ModelError", "CheckpointError", "WalError", "TokenizerError",
@@ -34,6 +36,7 @@ __all__ = [
     "Config", "Model", "KvCache", "Session", "DeferCheckpoint", "WalHeader", "WalWriter", "WalLog",
     "seed_from_u64", "chacha8_words", "words_per_sample", "sample_logits", "log_softmax_at",
     "ablation_attribution", "replay_batch", "generate_batch",
+    "Q8Cache", "q8_append", "q8_read", "q8_attend",
 ]
 
 
@@ -95,6 +98,9 @@ def _check(rc: int):
     if rc != 0:
         msg = (_L().defer_last_error() or b"").decode(errors="replace")
         raise _ERRORS.get(rc, DeferError)(msg)
+
+
+q8._check, q8._invalid = _check, InvalidArgumentError
 
 
 def _u8(b: bytes):

@@ -45,6 +45,20 @@ class WalHeaderC(ctypes.Structure):
                 ("prefix_tokens", c_u32p), ("n_prefix", sz)]
 
 
+class Q8CacheC(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int32), ("kind", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("slots", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("cap", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("k_codes", vp), ("v_codes", vp), ("k_scales", vp),
+                ("v_scales", vp), ("k_tail", vp), ("v_tail", vp)]
+
+
+class Q8BatchC(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("max_q", ctypes.c_uint32),
+                ("q_start", vp), ("slots", vp), ("status", vp)]
+
+
+i64, u32 = ctypes.c_int64, ctypes.c_uint32
+
 TOKEN_CB = ctypes.CFUNCTYPE(ctypes.c_int, vp, ctypes.c_uint32, ctypes.c_uint64)
 
 # (name, restype, argtypes) of every entry point declared in the header.
@@ -110,6 +124,11 @@ SIGNATURES = [
     ("defer_debug_stall", ctypes.c_int, [vp, ctypes.c_uint32]),
     ("defer_debug_tc_gemm", ctypes.c_int, [ctypes.c_int, c_f32p, ctypes.c_uint32, c_f32p, ctypes.c_uint32,
                                            ctypes.c_uint32, ctypes.c_int32, c_f32p]),
+    ("defer_q8_append", ctypes.c_int, [vp, vp, vp, vp, i64, i64, vp, i64, i64, vp]),
+    ("defer_q8_read", ctypes.c_int, [vp, u32, vp, vp, vp, vp, u32, vp, ctypes.POINTER(i64), vp, ctypes.POINTER(i64),
+                                     vp]),
+    ("defer_q8_attend", ctypes.c_int, [vp, vp, vp, u32, u32, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.c_int32,
+                                       ctypes.c_float, vp]),
     ("defer_log_softmax_at", ctypes.c_double, [c_f32p, sz, sz]),
 ]
 

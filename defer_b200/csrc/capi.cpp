@@ -2,10 +2,13 @@
 // mapping to status codes, and thin wrappers over the engine.
 #include "../../include/defer_b200.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <functional>
 #include <memory>
+#include <utility>
+#include <vector>
 
 #include "common.h"
 #include "engine.h"
@@ -14,6 +17,7 @@
 #include "hostutil.h"
 #include "kernels.h"
 #include "model.h"
+#include "q8.h"
 
 struct defer_model {
   std::unique_ptr<defer::Model> m;
@@ -66,6 +70,66 @@ void put_bytes(const std::vector<uint8_t>& v, uint8_t* buf, size_t cap, size_t* 
   if (!buf) return;
   if (cap < v.size()) defer::fail(defer::kInvalidArgument, "buffer too small");
   memcpy(buf, v.data(), v.size());
+}
+
+// The calling thread's device for the length of a call on caller's buffers.
+struct OnDevice {
+  int prev = 0;
+  explicit OnDevice(int device) {
+    DEFER_CUDA(cudaGetDevice(&prev));
+    if (device != prev) DEFER_CUDA(cudaSetDevice(device));
+  }
+  ~OnDevice() { cudaSetDevice(prev); }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+};
+
+void q8_check(bool ok, const char* what) {
+  if (!ok) defer::fail(defer::kInvalidArgument, std::string("8-bit cache: ") + what);
+}
+
+defer::Q8View q8_view(const defer_q8_cache* c) {
+  need(c, "cache");
+  for (const void* p : {(const void*)c->k_codes, (const void*)c->v_codes, (const void*)c->k_scales,
+                        (const void*)c->v_scales, (const void*)c->k_tail, (const void*)c->v_tail}) {
+    need(p, "cache buffer");
+    q8_check(reinterpret_cast<uintptr_t>(p) % 16 == 0, "buffers must be 16-byte aligned");
+  }
+  q8_check(c->device >= 0, "device must not be negative");
+  q8_check(c->kind == defer::kQ8Int8 || c->kind == defer::kQ8E4m3, "kind must be 0 (int8) or 1 (e4m3)");
+  q8_check(c->dtype >= defer::kQ8F32 && c->dtype <= defer::kQ8F16, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  q8_check(c->head_dim >= 16 && c->head_dim <= defer::kQ8MaxHeadDim && c->head_dim % 16 == 0,
+           "head_dim must be a multiple of 16 from 16 to 256");
+  q8_check(c->cap >= 16 && c->cap % 16 == 0 && c->cap <= 1u << 30, "cap must be a multiple of 16 up to 2^30");
+  q8_check(c->slots >= 1 && c->slots <= 1u << 24, "slots must be 1 to 2^24");
+  q8_check(c->kv_heads >= 1 && c->kv_heads <= 1024, "kv_heads must be 1 to 1024");
+  return {static_cast<unsigned char*>(c->k_codes), static_cast<unsigned char*>(c->v_codes), c->k_scales, c->v_scales,
+          c->k_tail, c->v_tail, (int)c->slots, (int)c->kv_heads, (int)c->cap, (int)c->head_dim, c->kind, c->dtype};
+}
+
+defer::Q8Batch q8_batch(const defer::Q8View& c, const defer_q8_batch* b) {
+  need(b, "batch");
+  q8_check(b->n <= 1u << 24 && b->tokens <= 1u << 30, "n must be at most 2^24, tokens at most 2^30");
+  q8_check(b->n > 0 || b->tokens == 0 || b->q_start, "rows without sequences");
+  if (!b->q_start && b->n) q8_check(b->tokens % b->n == 0, "without q_start every sequence has tokens / n rows");
+  if (!b->slots) q8_check(b->n <= (uint32_t)c.slots, "more sequences than slots");
+  uint32_t mq = b->max_q ? std::min(b->max_q, b->tokens) : b->tokens;
+  if (!b->q_start && b->n) mq = b->tokens / b->n;
+  return {(int)b->n, (int)b->tokens, (int)mq, b->q_start, b->slots, b->status};
+}
+
+// Whether rows of `len` elements at strides (count, stride) overlap.
+bool q8_overlap(int64_t len, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
+  std::vector<std::pair<int64_t, int64_t>> d;  // (stride, count)
+  for (const auto& x : dims)
+    if (x.first > 1) d.push_back({x.second, x.first});
+  std::sort(d.begin(), d.end());
+  int64_t extent = len;
+  for (const auto& x : d) {
+    if (x.first < extent) return true;
+    extent += x.first * (x.second - 1);
+  }
+  return false;
 }
 
 }  // namespace
@@ -626,6 +690,67 @@ int defer_debug_stall(defer_model* m, uint32_t wait_us) {
     if (wait_us == 0 || wait_us > 10000000u) defer::fail(defer::kInvalidArgument, "wait_us must be in 1..10^7");
     m->m->dbg_stall = 1;
     m->m->dbg_wait_ns = (unsigned long long)wait_us * 1000ull;
+  });
+}
+
+int defer_q8_append(const defer_q8_cache* cache, const defer_q8_batch* batch, const int32_t* pos, const void* k,
+                    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                    int64_t v_head_stride, void* stream) {
+  return guard([&] {
+    const defer::Q8View c = q8_view(cache);
+    const defer::Q8Batch b = q8_batch(c, batch);
+    if (b.n == 0 || b.tokens == 0) return;
+    need(pos, "pos");
+    need(k, "k");
+    need(v, "v");
+    OnDevice on(cache->device);
+    defer::q8_append(c, b, pos, {k, k_token_stride, k_head_stride}, {v, v_token_stride, v_head_stride},
+                     static_cast<cudaStream_t>(stream));
+  });
+}
+
+int defer_q8_read(const defer_q8_cache* cache, uint32_t n, const int32_t* lens, const int32_t* start,
+                  const int32_t* slots, int32_t* status, uint32_t rows, void* k_out, const int64_t k_strides[3],
+                  void* v_out, const int64_t v_strides[3], void* stream) {
+  return guard([&] {
+    const defer::Q8View c = q8_view(cache);
+    q8_check(n <= 1u << 24 && rows <= 1u << 30, "n must be at most 2^24, rows at most 2^30");
+    if (!slots) q8_check(n <= (uint32_t)c.slots, "more sequences than slots");
+    if (n == 0 || rows == 0) return;
+    need(lens, "lens");
+    need(k_out, "k_out");
+    need(v_out, "v_out");
+    need(k_strides, "k_strides");
+    need(v_strides, "v_strides");
+    for (const int64_t* s : {k_strides, v_strides})
+      q8_check(!q8_overlap(c.hd, {{n, s[0]}, {c.kvh, s[1]}, {rows, s[2]}}), "the output's rows overlap");
+    OnDevice on(cache->device);
+    defer::q8_read(c, (int)n, lens, start, slots, status, (int)rows, {k_out, k_strides[0], k_strides[2], k_strides[1]},
+                   {v_out, v_strides[0], v_strides[2], v_strides[1]}, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int defer_q8_attend(const defer_q8_cache* cache, const defer_q8_batch* batch, const int32_t* lens, uint32_t max_len,
+                    uint32_t heads, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                    int64_t out_token_stride, int64_t out_head_stride, const uint8_t* masked, int64_t mask_stride,
+                    int32_t causal, float scale, void* stream) {
+  return guard([&] {
+    const defer::Q8View c = q8_view(cache);
+    const defer::Q8Batch b = q8_batch(c, batch);
+    q8_check(heads >= 1 && heads % (uint32_t)c.kvh == 0 && heads <= 16384, "heads must be a multiple of kv_heads");
+    q8_check(std::isfinite(scale), "scale must be finite");
+    q8_check(!masked || mask_stride == 0 || mask_stride >= c.cap, "masked must have a byte for each of cap positions");
+    if (b.n == 0 || b.tokens == 0) return;
+    need(lens, "lens");
+    need(q, "q");
+    need(out, "out");
+    q8_check(!q8_overlap(c.hd, {{b.tokens, out_token_stride}, {heads, out_head_stride}}), "the output's rows overlap");
+    const int most = max_len ? (int)std::min<uint32_t>(max_len, (uint32_t)c.cap) : c.cap;
+    OnDevice on(cache->device);
+    defer::q8_attend(c, b,
+                     {lens, most, (int)heads, {q, q_token_stride, q_head_stride}, {out, out_token_stride, out_head_stride},
+                      masked, mask_stride, causal != 0, scale},
+                     static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -1,0 +1,80 @@
+// Key/value cache in 8 bits: host entry points of the kernels in q8.cu.
+//
+// One layer of a cache is held in the caller's device memory as
+//   codes  [slots][kv_heads][cap][head_dim]  int8 or e4m3, for K and for V
+//   scales [slots][kv_heads][cap / 16]       fp32, one per block and head
+//   tail   [slots][kv_heads][16][head_dim]   the open block's tokens as given
+// A block of 16 tokens is quantised when its last token arrives, so its
+// codes depend on its tokens alone (not on how many came in one call) and no
+// value is rounded twice.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace defer {
+
+constexpr int kQ8Block = 16;        // tokens that share a scale
+constexpr int kQ8MaxHeadDim = 256;  // head_dim is a multiple of 16 up to this
+
+enum Q8Kind : int { kQ8Int8 = 0, kQ8E4m3 = 1 };
+enum Q8Type : int { kQ8F32 = 0, kQ8Bf16 = 1, kQ8F16 = 2 };
+
+// Bits of the optional status word (a sequence that sets one is skipped).
+enum Q8Status : int {
+  kQ8BadRange = 1,   // slot, length, position or row range outside its bounds
+  kQ8SlotTwice = 2,  // append: the slot appears in an earlier sequence of the call
+};
+
+// One layer's buffers (every pointer 16-byte aligned device memory).
+struct Q8View {
+  unsigned char *kc, *vc;
+  float *ks, *vs;
+  void *kt, *vt;
+  int slots, kvh, cap, hd;
+  int kind, type;
+};
+
+// The rows of a call: sequence i has rows [q_start[i], q_start[i + 1]) of
+// the k/v or q/out arrays (q_start null: tokens / n rows each) and is held
+// in slot slots[i] (null: slot i; negative: skipped, its rows left alone).
+struct Q8Batch {
+  int n, tokens;
+  int max_q;  // rows of the longest sequence (sizes the grid only)
+  const int* q_start;
+  const int* slots;
+  int* status;  // or null
+};
+
+// Strides in elements; the head_dim elements of a row are contiguous.
+struct Q8Rows {
+  const void* p;
+  int64_t token, head;
+};
+
+void q8_append(const Q8View& c, const Q8Batch& b, const int* pos, const Q8Rows& k, const Q8Rows& v, cudaStream_t st);
+
+// Positions [start, min(len, start + rows)) of each sequence to output rows
+// 0, 1, ...; rows behind them stay as they are.
+struct Q8Out {
+  void* p;
+  int64_t seq, token, head;
+};
+void q8_read(const Q8View& c, int n, const int* lens, const int* start, const int* slots, int* status, int rows,
+             const Q8Out& k, const Q8Out& v, cudaStream_t st);
+
+struct Q8Attend {
+  const int* lens;
+  int max_len;  // longest sequence (sizes the grid only)
+  int heads;
+  Q8Rows q;
+  Q8Rows out;  // p is written
+  const unsigned char* masked;  // [n][mask_stride] nonzero hides a position, or null
+  int64_t mask_stride;
+  int causal;
+  float scale;
+};
+void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st);
+
+}  // namespace defer

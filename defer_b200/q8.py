@@ -1,0 +1,195 @@
+"""Key/value cache in 8 bits on the caller's device buffers: defer_q8_append,
+defer_q8_read and defer_q8_attend of include/defer_b200.h for arrays that
+have a device pointer (torch CUDA tensors; torch itself is not imported).
+
+    cache = Q8Cache(k_codes, v_codes, k_scales, v_scales, k_tail, v_tail)
+    q8_append(cache, k, v, pos)             # rows into the cache
+    q8_attend(cache, q, out, lens)          # attention over it
+    q8_read(cache, k_out, v_out, lens)      # values back
+
+Every call launches on `stream` (a cudaStream_t as an integer), by default
+torch's current stream of the cache's device, allocates nothing on the device
+and waits for nothing, so it may be captured into a CUDA graph. The arrays
+must stay allocated until the stream has run the call.
+"""
+from __future__ import annotations
+
+import ctypes
+import sys
+from typing import Optional
+
+from . import _lib
+
+BLOCK = 16  # positions that share a scale
+_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+_KINDS = {"torch.int8": 0, "torch.float8_e4m3fn": 1}
+_BYTES = ("torch.uint8", "torch.bool", "torch.int8")
+_I64x3 = ctypes.c_int64 * 3
+_check = None  # the package's status check (set by defer_b200/__init__.py)
+_invalid = None
+
+
+def _refuse(what: str):
+    raise _invalid("8-bit cache: " + what)
+
+
+def _stream_of(device: int) -> int:
+    t = sys.modules.get("torch")
+    return t.cuda.current_stream(device).cuda_stream if t is not None else 0
+
+
+_names = {}  # dtype object -> its name (str() of a torch dtype costs more than a call's other checks)
+
+
+def _name(x) -> str:
+    try:
+        return _names[x.dtype]
+    except KeyError:
+        return _names.setdefault(x.dtype, str(x.dtype))
+
+
+def _dense(x, what: str):
+    if not x.is_contiguous():
+        _refuse(f"{what} must be contiguous")
+
+
+class Q8Cache:
+    """One layer of a cache: codes [slots, kv_heads, cap, head_dim] (int8 or
+    float8_e4m3fn), scales [slots, kv_heads, cap / 16] (float32) and the open
+    blocks' tokens, tail [slots, kv_heads, 16, head_dim] (float32, bfloat16 or
+    float16), for K and V. The arrays are the caller's and are kept alive."""
+
+    __slots__ = ("k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail", "slots", "kv_heads", "cap",
+                 "head_dim", "device", "dtype", "_c", "_ref")
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales, k_tail, v_tail):
+        if len(k_codes.shape) != 4:
+            _refuse("codes are [slots, kv_heads, cap, head_dim]")
+        s, h, cap, hd = (int(x) for x in k_codes.shape)
+        kind, dtype = _KINDS.get(_name(k_codes)), _DTYPES.get(_name(k_tail))
+        if kind is None:
+            _refuse(f"codes are int8 or float8_e4m3fn, got {_name(k_codes)}")
+        if dtype is None:
+            _refuse(f"tails are float32, bfloat16 or float16, got {_name(k_tail)}")
+        if cap % BLOCK:
+            _refuse("cap must be a multiple of 16")
+        dev = k_codes.get_device() if k_codes.is_cuda else -1
+        for x, shape, name, what in ((k_codes, (s, h, cap, hd), _name(k_codes), "k_codes"),
+                                     (v_codes, (s, h, cap, hd), _name(k_codes), "v_codes"),
+                                     (k_scales, (s, h, cap // BLOCK), "torch.float32", "k_scales"),
+                                     (v_scales, (s, h, cap // BLOCK), "torch.float32", "v_scales"),
+                                     (k_tail, (s, h, BLOCK, hd), _name(k_tail), "k_tail"),
+                                     (v_tail, (s, h, BLOCK, hd), _name(k_tail), "v_tail")):
+            if tuple(x.shape) != shape or _name(x) != name:
+                _refuse(f"{what} must be {name} {shape}, got {_name(x)} {tuple(x.shape)}")
+            _dense(x, what)
+            if not x.is_cuda or x.get_device() != dev:
+                _refuse(f"{what} must be on the cache's CUDA device")
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
+        self.k_tail, self.v_tail = k_tail, v_tail
+        self.slots, self.kv_heads, self.cap, self.head_dim = s, h, cap, hd
+        self.device, self.dtype = dev, k_tail.dtype
+        self._c = _lib.Q8CacheC(dev, kind, dtype, s, h, cap, hd, k_codes.data_ptr(), v_codes.data_ptr(),
+                                k_scales.data_ptr(), v_scales.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr())
+        self._ref = ctypes.addressof(self._c)
+
+
+def _ints(cache: Q8Cache, x, n: Optional[int], what: str):
+    """Device pointer of an int32 array of n entries (None: NULL)."""
+    if x is None:
+        return None
+    if _name(x) != "torch.int32" or (n is not None and x.numel() != n) or not x.is_contiguous():
+        _refuse(f"{what} must be {n} contiguous int32")
+    if x.get_device() != cache.device:
+        _refuse(f"{what} must be on the cache's device")
+    return x.data_ptr()
+
+
+def _rows(cache: Q8Cache, x, heads: int, what: str):
+    """(pointer, row stride, head stride) of [tokens, heads, head_dim]."""
+    shape = x.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != cache.head_dim or x.dtype != cache.dtype:
+        _refuse(f"{what} must be {cache.dtype} [tokens, {heads}, {cache.head_dim}], got {x.dtype} {tuple(shape)}")
+    if x.get_device() != cache.device:
+        _refuse(f"{what} must be on the cache's device")
+    st = x.stride()
+    if st[2] != 1:
+        _refuse(f"the head_dim elements of {what} must be contiguous")
+    return x.data_ptr(), st[0], st[1]
+
+
+def q8_append(cache: Q8Cache, k, v, pos, *, q_start=None, slots=None, max_q: int = 0, status=None,
+              stream: Optional[int] = None) -> None:
+    """Writes rows k, v [tokens, kv_heads, head_dim] at positions pos[i],
+    pos[i] + 1, ... of each sequence i (defer_q8_append). pos, q_start, slots
+    and status are int32 device arrays."""
+    n = pos.numel()
+    kp, kt, kh = _rows(cache, k, cache.kv_heads, "k")
+    vp, vt, vh = _rows(cache, v, cache.kv_heads, "v")
+    tokens = k.shape[0]
+    if v.shape[0] != tokens:
+        _refuse("k and v must have the same rows")
+    b = _lib.Q8BatchC(n, tokens, max_q, _ints(cache, q_start, n + 1, "q_start"), _ints(cache, slots, n, "slots"),
+                      _ints(cache, status, None, "status"))
+    rc = _lib.load().defer_q8_append(cache._ref, ctypes.addressof(b), _ints(cache, pos, n, "pos"), kp, kt, kh, vp, vt,
+                                     vh, _stream_of(cache.device) if stream is None else stream)
+    if rc:
+        _check(rc)
+
+
+def q8_read(cache: Q8Cache, k_out, v_out, lens, *, start=None, slots=None, status=None,
+            stream: Optional[int] = None) -> None:
+    """Positions start[i] .. lens[i] - 1 of each sequence into k_out and v_out
+    [n, kv_heads, rows, head_dim] (any strides of the first three); rows
+    behind the last position are left as they were (defer_q8_read)."""
+    n = lens.numel()
+    shape = tuple(k_out.shape)
+    if len(shape) != 4 or shape[0] != n or shape[1] != cache.kv_heads or shape[3] != cache.head_dim:
+        _refuse(f"k_out must be [{n}, {cache.kv_heads}, rows, {cache.head_dim}], got {shape}")
+    if tuple(v_out.shape) != shape:
+        _refuse("k_out and v_out must have the same shape")
+    for x, what in ((k_out, "k_out"), (v_out, "v_out")):
+        if x.dtype != cache.dtype or x.get_device() != cache.device:
+            _refuse(f"{what} must be {cache.dtype} on the cache's device")
+        if x.stride(3) != 1:
+            _refuse(f"the head_dim elements of {what} must be contiguous")
+    rc = _lib.load().defer_q8_read(cache._ref, n, _ints(cache, lens, n, "lens"), _ints(cache, start, n, "start"),
+                                   _ints(cache, slots, n, "slots"), _ints(cache, status, None, "status"), shape[2],
+                                   k_out.data_ptr(), _I64x3(*k_out.stride()[:3]), v_out.data_ptr(),
+                                   _I64x3(*v_out.stride()[:3]),
+                                   _stream_of(cache.device) if stream is None else stream)
+    if rc:
+        _check(rc)
+
+
+def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: int = 0, max_len: int = 0,
+              masked=None, causal: bool = True, scale: Optional[float] = None, status=None,
+              stream: Optional[int] = None):
+    """Attention of q [tokens, heads, head_dim] over the cache into out (the
+    same shape), which is returned (defer_q8_attend). lens[i] counts the
+    positions of sequence i, the call's own rows among them; masked [n, cap or
+    more] (uint8 or bool) hides positions; scale defaults to
+    head_dim ** -0.5."""
+    n = lens.numel()
+    heads = q.shape[1] if len(q.shape) == 3 else 0
+    qp, qt, qh = _rows(cache, q, heads, "q")
+    op, ot, oh = _rows(cache, out, heads, "out")
+    tokens = q.shape[0]
+    if out.shape[0] != tokens:
+        _refuse("q and out must have the same rows")
+    mp, ms = None, 0
+    if masked is not None:
+        if len(masked.shape) != 2 or masked.shape[0] != n or masked.shape[1] < cache.cap or _name(masked) not in _BYTES:
+            _refuse(f"masked must be uint8 or bool [{n}, at least {cache.cap}]")
+        if masked.stride(1) != 1 or masked.get_device() != cache.device:
+            _refuse("masked must be on the cache's device with contiguous rows")
+        mp, ms = masked.data_ptr(), masked.stride(0) if n > 1 else 0
+    b = _lib.Q8BatchC(n, tokens, max_q, _ints(cache, q_start, n + 1, "q_start"), _ints(cache, slots, n, "slots"),
+                      _ints(cache, status, None, "status"))
+    rc = _lib.load().defer_q8_attend(cache._ref, ctypes.addressof(b), _ints(cache, lens, n, "lens"), max_len, heads,
+                                     qp, qt, qh, op, ot, oh, mp, ms, 1 if causal else 0,
+                                     cache.head_dim ** -0.5 if scale is None else scale,
+                                     _stream_of(cache.device) if stream is None else stream)
+    if rc:
+        _check(rc)
+    return out

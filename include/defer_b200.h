@@ -265,6 +265,86 @@ DEFER_API int defer_debug_tc_gemm(int device, const float* x, uint32_t m, const 
 /* attribution::log_softmax_at (src/attribution.rs:71-85). */
 DEFER_API double defer_log_softmax_at(const float* logits, size_t n, size_t idx);
 
+/* -------------------------------------------- key/value cache in 8 bits --- */
+/* No counterpart in the reference, whose cache is fp32 (src/model.rs:184-243):
+ * a cache of a quarter of the bytes, for callers whose sessions no longer fit
+ * or whose steps are bound by reading the cache. These operators work on the
+ * caller's own device buffers (as defer_forward_noalloc does), allocate
+ * nothing, synchronise nothing and may be captured into a CUDA graph; calls
+ * that write one cache must be ordered by the caller (one stream, events).
+ *
+ * One layer of the cache, every pointer 16-byte aligned memory of `device`:
+ *   codes  [slots][kv_heads][cap][head_dim]   int8 (kind 0) or e4m3 (kind 1)
+ *   scales [slots][kv_heads][cap / 16]        float
+ *   tail   [slots][kv_heads][16][head_dim]    `dtype`: 0 float, 1 bf16, 2 fp16
+ * for K and for V. cap is a multiple of 16, head_dim a multiple of 16 up to
+ * 256. Blocks of 16 positions share one scale per head: a block is quantised
+ * when its 16th position is written, with s = max|x| / Q (Q = 127 or 448) and
+ * code = round(x * (1 / s)) in fp32 (s = 0 when max|x| < 2^-117); until then
+ * its positions are held as given in the tail. So codes do not depend on how
+ * many positions came in one call. An 8-bit code holds no NaN and no infinity:
+ * when a block closes, the maximum is taken over its finite values, a NaN is
+ * stored as 0 and an infinity as +-Q. The block of position len / 16 is the
+ * open one of a sequence of len positions: to shorten a sequence, shorten it
+ * inside that block, or to a multiple of 16. */
+typedef struct {
+  int32_t device, kind, dtype;
+  uint32_t slots, kv_heads, cap, head_dim;
+  void *k_codes, *v_codes;
+  float *k_scales, *v_scales;
+  void *k_tail, *v_tail;
+} defer_q8_cache;
+
+/* The sequences of a call. Sequence i has rows q_start[i] .. q_start[i + 1]
+ * - 1 of the `tokens` rows of k/v or q/out (q_start NULL: tokens / n rows
+ * each; rows behind q_start[n] are left as they were) and lives in slot
+ * slots[i] (NULL: slot i; negative: the sequence is skipped and its rows are
+ * left as they were). max_q: the largest number of rows of a sequence (0:
+ * tokens); it sizes the launch and changes no result of defer_q8_append.
+ * q_start, slots and status are device memory. A sequence whose slot, rows,
+ * position or length is out of range is skipped (defer_q8_attend fills its
+ * rows with NaN where the rows themselves are valid), as is, when appending,
+ * one whose slot an earlier sequence of the call names; if `status` is not
+ * NULL the kernel then sets bit 0 (range) or bit 1 (slot named twice) in it. */
+typedef struct {
+  uint32_t n, tokens, max_q;
+  const int32_t* q_start;
+  const int32_t* slots;
+  int32_t* status;
+} defer_q8_batch;
+
+/* Writes rows k and v [tokens][kv_heads][head_dim] of the cache's dtype
+ * (strides of rows and heads in elements) at positions pos[i], pos[i] + 1, ...
+ * of each sequence; pos [n] is device memory. The cache holds pos[i]
+ * positions already, those of the open block in the tail. */
+DEFER_API int defer_q8_append(const defer_q8_cache* c, const defer_q8_batch* b, const int32_t* pos, const void* k,
+                              int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                              int64_t v_head_stride, void* stream);
+/* Reads positions start[i] .. len - 1 (at most `rows`; start NULL: from 0)
+ * of sequence i of lens[i] positions back: value = code * scale rounded once
+ * to the cache's dtype, or the open block's value as given, to k_out and
+ * v_out [n][kv_heads][rows][head_dim] with the element strides
+ * {sequence, head, row}; rows behind the last position are left as they were.
+ * slots and status as in defer_q8_batch. */
+DEFER_API int defer_q8_read(const defer_q8_cache* c, uint32_t n, const int32_t* lens, const int32_t* start,
+                            const int32_t* slots, int32_t* status, uint32_t rows, void* k_out,
+                            const int64_t k_strides[3], void* v_out, const int64_t v_strides[3], void* stream);
+/* Attention of q [tokens][heads][head_dim] over the cache into out, both of
+ * the cache's dtype: head h reads key head h / (heads / kv_heads). lens[i] is
+ * the length of sequence i with the call's own rows appended: with `causal`
+ * row j of a sequence of r rows sees positions 0 .. lens[i] - r + j, else all
+ * lens[i]. masked (NULL, or device bytes [n] with row stride mask_stride, 0 or
+ * at least cap): position t of sequence i is hidden where masked[i *
+ * mask_stride + t] is not 0. out = sum_t p_t V_t, p = softmax(scale * q . K_t)
+ * over the positions seen, 0 when there are none; softmax and sums in fp32.
+ * max_len: the longest length (0: cap); it sizes the launch. A sequence's
+ * result depends on its own rows, length and cache only, not on the call's
+ * other sequences. */
+DEFER_API int defer_q8_attend(const defer_q8_cache* c, const defer_q8_batch* b, const int32_t* lens,
+                              uint32_t max_len, uint32_t heads, const void* q, int64_t q_token_stride,
+                              int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                              const uint8_t* masked, int64_t mask_stride, int32_t causal, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
