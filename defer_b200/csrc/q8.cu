@@ -271,93 +271,573 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 }
 
 // ------------------------------------------------------------------ attend
-// One CTA per query row and head: pieces of 128 positions, a score a thread,
-// then the weighted values a dimension (or two) a thread, with the running
-// maximum and sum of the softmax.
-template <int TYPE, int KIND>
-__global__ void __launch_bounds__(128) k_q8_attend(Q8View c, Q8Batch b, Q8Attend a) {
+// Attention of a few rows (q8_few_rows) of a sequence and key head: the cache
+// is read once, and everything else is arranged around that stream.
+//
+// Mathematics. A code is a whole number (or an e4m3 number): exact in fp16,
+// so the scores of a block are (codes . q) * s_K and its share of the output
+// is (P . codes) * s_V with the scales outside the products, which run on the
+// tensor cores (mma m16n8k16, fp32 sums). The other operand is made as exact
+// as the cache's type asks: a q row is scaled by a power of two so that its
+// largest element is in [2^14, 2^15) and held as one fp16 term (bf16 and fp16
+// rows: no bit lost) or two (fp32: 22 bits); P is kept times 2^15, so that
+// weights down to 2^-29 of the largest are full fp16 numbers, and held the
+// same way. Products of one block of 16 positions are summed by the tensor
+// core from zero and added to the running sums in fp32 registers: long chains
+// inside the tensor core lose bits. Softmax: running maximum and sum per warp
+// in base 2; warps, then splits, are merged in order.
+//
+// Work. The positions of the closed blocks are cut into units of 8 warp
+// steps, the units into splits, one CTA each, the splits of a (sequence, key
+// head, row tile) forming a cluster: partial results travel through
+// distributed shared memory, so the call needs no workspace and no second
+// launch. The number of splits follows from the sequence's length alone, so
+// its result does not depend on the batch it runs in. Each warp streams its
+// own steps (4 KB of K and V) through a ring of its own with 16-byte
+// asynchronous copies, without any barrier; chunks are swizzled so that both
+// the row-wise reads of K and the column-wise reads of V are free of bank
+// conflicts. The open block (fp32 or 16-bit tokens) is added at the end by
+// the last split, a token a warp, in fp32.
+constexpr int kQsWarps = 8;
+constexpr int kQsMaxSplits = 16;
+
+template <int HDP>
+struct QsShape {
+  static constexpr int TS = HDP >= 128 ? 16 : 2048 / HDP;  // positions of a warp step
+  static constexpr int NG = TS / kQ8Block;                 // blocks of a step
+  static constexpr int CH = HDP / 16;                      // 16-byte chunks of a row
+  static constexpr int KS = HDP / 16;                      // k steps of the score product
+  static constexpr int STAGES = HDP == 256 ? 2 : 3;
+  static constexpr int KBYTES = TS * HDP;
+  static constexpr int STAGE = 2 * KBYTES + 2 * NG * 4 + (32 - 2 * NG * 4 % 32) % 32;  // codes, scales, pad
+  static constexpr int UNIT = kQsWarps * TS;               // positions of one step of the CTA
+  static constexpr int ORow = HDP + 4;                     // floats of a result row
+};
+template <int HDP, int NT, int QT>
+constexpr size_t qs_smem() {
+  using S = QsShape<HDP>;
+  return (size_t)kQsWarps * S::STAGES * S::STAGE          // rings (later the warps' results)
+         + (size_t)S::KS * NT * QT * 32 * 8               // q
+         + (size_t)(8 * NT) * S::ORow * 4                 // the CTA's result
+         + (size_t)(8 * NT) * (3 + 2 * kQsWarps) * 4;     // row factors, m and l of the CTA and of the warps
+}
+
+// Splits of a sequence with `closed` positions in closed blocks.
+template <int HDP>
+__host__ __device__ __forceinline__ int qs_splits(int closed) {
+  const int units = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT;
+  return units < 1 ? 1 : units > kQsMaxSplits ? kQsMaxSplits : units;
+}
+
+// Byte offset of 16-byte chunk `ch` of position `t` in a step's K or V. The
+// exclusive-or keeps a 128-byte phase of both access patterns on 32 banks: K
+// is read by 8 threads as 2 neighbouring rows x 4 chunks (or whole rows), V as
+// rows 2c (or 2c + 1), c = 0..3, x neighbouring chunks.
+template <int HDP>
+__device__ __forceinline__ int qs_chunk(int t, int ch) {
+  if constexpr (HDP == 256) return t * 256 + ((ch ^ ((t >> 1 & 1) | (((t >> 2) ^ t) & 1) << 2)) << 4);
+  else if constexpr (HDP == 128) return t * 128 + ((ch ^ ((t & 6) ^ (t & 1) << 2)) << 4);
+  else if constexpr (HDP == 64) return (t >> 1) * 128 + ((((t & 1) * 4 + ch) ^ ((t >> 1 & 3) * 2)) << 4);
+  else return (t >> 2) * 128 + ((((t & 3) * 2 + ch) ^ ((t >> 2 & 1) * 2)) << 4);
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 of 16 bits across the warp
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp16 numbers from code bytes (SEL: the prmt selector that puts two
+// bytes x, y as x . y . into 16-bit lanes). int8: the byte with its sign bit
+// flipped is x + 128; 0x6400 | u is 1024 + u, so one subtraction of 1152
+// leaves x, exactly. `w` comes from flip<KIND>.
+template <int KIND>
+__device__ __forceinline__ uint32_t flip(uint32_t w) {
+  return KIND == kQ8Int8 ? w ^ 0x80808080u : w;
+}
+template <int KIND, bool HI>
+__device__ __forceinline__ uint32_t halves(uint32_t w) {
+  if constexpr (KIND == kQ8Int8) {
+    const uint32_t u = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
+    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480))));
+  } else {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? w >> 16 : w & 0xFFFFu), __NV_E4M3);
+    return h2_bits(__half2(h));
+  }
+}
+
+__device__ __forceinline__ void cluster_arrive_wait() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+// This CTA's shared address `a` in the CTA of cluster rank `r`.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t a, uint32_t r) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(r));
+  return d;
+}
+__device__ __forceinline__ float ld_peer(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// Weight of a partial result with maximum m under the total's maximum M.
+__device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(m - M); }
+
+template <int TYPE, int KIND, int HDP, int NT>
+__global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
+    k_q8_attend(const __grid_constant__ Q8View c, const __grid_constant__ Q8Batch b, const __grid_constant__ Q8Attend a,
+                int tiles) {
+  using S = QsShape<HDP>;
   using E = Elem<TYPE>;
   using T = typename E::T;
-  __shared__ float qs[kQ8MaxHeadDim], ps[128], red[4];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x, head = blockIdx.y, hd = c.hd;
-  int i;
-  if (b.q_start) {
-    int lo = 0, hi = b.n;  // the last i with q_start[i] <= row
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (__ldg(b.q_start + mid) <= row) lo = mid;
-      else hi = mid;
-    }
-    i = lo;
-  } else {
-    i = row / (b.tokens / b.n);
-  }
+  constexpr int QT = TYPE == kQ8F32 ? 2 : 1, ROWS = 8 * NT, MT = HDP / 16, KW = HDP / 16;
+  extern __shared__ __align__(128) unsigned char sm[];
+  uint2* qf = reinterpret_cast<uint2*>(sm + (size_t)kQsWarps * S::STAGES * S::STAGE);
+  float* res = reinterpret_cast<float*>(qf + S::KS * NT * QT * 32);  // [ROWS][ORow]
+  float* fac = res + ROWS * S::ORow;                                  // [ROWS] row factors
+  float* cm = fac + ROWS;                                             // [ROWS] the CTA's m, then l
+  float* wm = cm + 2 * ROWS;                                          // [warps][ROWS] m, then [warps][ROWS] l
+  float* wl = wm + kQsWarps * ROWS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, cq = lane & 3;
+  const int csize = (int)cluster_size(), rank = (int)cluster_rank();
+  const int i = blockIdx.x / csize;
+  const int kvh = blockIdx.y / tiles;
   const Seq s = seq_of(b, c.slots, i);
-  const int j = row - s.row0;
-  if (s.slot == kSeqSkip || j < 0 || j >= s.nrow) return;
+  const int G = a.heads / c.kvh, R = s.nrow * G;
+  // every CTA of a cluster takes the same way out
+  if (s.slot == kSeqSkip || R == 0) return;
   const int len = s.slot == kSeqBad ? -1 : __ldg(a.lens + i);
-  T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.token + (int64_t)head * a.out.head;
+  T* const out0 = static_cast<T*>(const_cast<void*>(a.out.p));
   if (len < 0 || len > c.cap) {
     if (b.status && tid == 0) atomicOr(b.status, (int)kQ8BadRange);
-    for (int d = tid; d < hd; d += 128) out[d] = E::from(NAN);
+    for (int x = (blockIdx.y - kvh * tiles) * csize + rank; x < R; x += tiles * csize)
+      for (int d = tid; d < c.hd; d += kQsWarps * 32)
+        out0[(int64_t)(s.row0 + x / G) * a.out.token + (int64_t)(kvh * G + x % G) * a.out.head + d] = E::from(NAN);
     return;
   }
-  const int seen = a.causal ? len - (s.nrow - 1 - j) : len;
-  const T* q = static_cast<const T*>(a.q.p) + (int64_t)row * a.q.token + (int64_t)head * a.q.head;
-  for (int d = tid; d < hd; d += 128) qs[d] = E::to(q[d]);
-  __syncthreads();
-  const size_t sh = (size_t)s.slot * c.kvh + head / (a.heads / c.kvh);
-  const int closed = len / kQ8Block * kQ8Block;
-  float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int t0 = 0; t0 < seen; t0 += 128) {
-    const int t = t0 + tid;
-    float sc = -INFINITY;
-    if (t < seen && !(a.masked && a.masked[(int64_t)i * a.mask_stride + t])) {
-      float dot = 0.0f;
-      if (t < closed) {
-        const unsigned char* k = c.kc + (sh * c.cap + t) * hd;
-        for (int d = 0; d < hd; d++) dot = fmaf(qs[d], decode<KIND>(k[d]), dot);
-        dot *= c.ks[sh * (c.cap / kQ8Block) + t / kQ8Block];
-      } else {
-        const T* k = static_cast<const T*>(c.kt) + (sh * kQ8Block + t - closed) * hd;
-        for (int d = 0; d < hd; d++) dot = fmaf(qs[d], E::to(k[d]), dot);
+  const int hd = c.hd, closed = len & ~(kQ8Block - 1);
+  const int ns = min(qs_splits<HDP>(closed), csize);
+  const size_t sh = (size_t)s.slot * c.kvh + kvh;
+  const unsigned char* kc = c.kc + sh * c.cap * hd;
+  const unsigned char* vc = c.vc + sh * c.cap * hd;
+  const float* ksc = c.ks + sh * (c.cap / kQ8Block);
+  const float* vsc = c.vs + sh * (c.cap / kQ8Block);
+  const unsigned char* hide = a.masked ? a.masked + (int64_t)i * a.mask_stride : nullptr;
+  unsigned char* ring = sm + (size_t)warp * S::STAGES * S::STAGE;
+  const uint32_t ring_u = smem_u32(ring);
+  const int units = (closed + S::UNIT - 1) / S::UNIT;
+
+  for (int tile = blockIdx.y - kvh * tiles; tile * ROWS < R; tile += tiles) {
+    const int x0 = tile * ROWS;
+    const int jlast = min(x0 + ROWS, R) - 1;
+    // positions that the tile's last row sees bound the work of the tile
+    const int most = a.causal ? min(len, len - (s.nrow - 1 - jlast / G)) : len;
+    const int least = a.causal ? len - (s.nrow - 1 - x0 / G) : len;  // the first row's
+    const int u0 = rank < ns ? (int)((int64_t)units * rank / ns) : 0;
+    const int u1 = rank < ns ? (int)((int64_t)units * (rank + 1) / ns) : 0;
+    const int t_end = min(min(closed, most), u1 * S::UNIT);
+    const int t_first = u0 * S::UNIT + warp * S::TS;
+
+    auto issue = [&](int t0, int st) {
+      if (t0 < t_end) {
+        const uint32_t base = ring_u + st * S::STAGE;
+#pragma unroll
+        for (int e = 0; e < S::TS * S::CH / 32; e++) {
+          const int x = e * 32 + lane, t = x / S::CH, ch = x % S::CH;
+          const bool on = t0 + t < closed && ch * 16 < hd;
+          const size_t o = on ? (size_t)(t0 + t) * hd + ch * 16 : 0;
+          const uint32_t d = base + qs_chunk<HDP>(t, ch);
+          cp16(d, kc + o, on);
+          cp16(d + S::KBYTES, vc + o, on);
+        }
+        if (lane < 2 * S::NG) {
+          const int g = lane % S::NG;
+          const bool on = t0 + g * kQ8Block < closed;
+          cp4(base + 2 * S::KBYTES + lane * 4, (lane < S::NG ? ksc : vsc) + (on ? t0 / kQ8Block + g : 0), on);
+        }
       }
-      sc = dot * a.scale;
+      cp_commit();
+    };
+#pragma unroll
+    for (int st = 0; st < S::STAGES - 1; st++) issue(t_first + st * S::UNIT, st);
+
+    // q rows of the tile as score operands: warp w takes rows w, w + 8
+    for (int x = warp; x < ROWS; x += kQsWarps) {
+      const bool on = x0 + x < R;
+      const T* q = static_cast<const T*>(a.q.p) + (int64_t)(s.row0 + (x0 + x) / G) * a.q.token +
+                   (int64_t)(kvh * G + (x0 + x) % G) * a.q.head;
+      float v[HDP / 32], mx = 0.0f;
+#pragma unroll
+      for (int e = 0; e < HDP / 32; e++) {
+        const int d = e * 32 + lane;
+        v[e] = on && d < hd ? E::to(q[d]) : 0.0f;
+        mx = fmaxf(mx, fabsf(v[e]));
+      }
+      mx = warp_max_all(mx);
+      // up = 2^(14 - exponent of mx); a zero, infinite or NaN row is not scaled
+      int ex = 0;
+      if (mx > 0.0f && mx <= FLT_MAX) {
+        frexpf(mx, &ex);  // mx in [2^(ex - 1), 2^ex)
+        ex = 15 - ex;
+      }
+      // the power is applied in two steps: 2^ex itself may exceed fp32's range
+      const float up0 = ldexpf(1.0f, ex / 2), up1 = ldexpf(1.0f, ex - ex / 2);
+      if (lane == 0) fac[x] = a.scale * 1.4426950408889634f / up0 / up1;
+#pragma unroll
+      for (int e = 0; e < HDP / 32; e++) {
+        const int d = e * 32 + lane;
+        const float y = v[e] * up0 * up1;
+        const int cc = HDP >= 64 ? d / 16 % 4 : d / 8, w = HDP >= 64 ? d % 16 / 4 : d % 8 / 4, bb = d % 4;
+        const int k = HDP >= 64 ? d / 64 * 4 + w : w;
+        __half* dst = reinterpret_cast<__half*>(qf + ((k * NT + x / 8) * QT) * 32 + (x % 8) * 4 + cc) + bb;
+        const __half hi = __float2half_rn(y);
+        dst[0] = hi;
+        if constexpr (QT == 2) {
+          // an infinite or NaN row keeps it in the first term
+          const float lo = y - __half2float(hi);
+          dst[32 * 4] = __float2half_rn(lo == lo ? lo : 0.0f);
+        }
+      }
     }
-    float mx = warp_max_all(sc);
-    if (lane == 0) red[warp] = mx;
     __syncthreads();
-    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mn = fmaxf(m, mx);
-    const float w = m == -INFINITY ? 0.0f : expf(m - mn);
-    ps[tid] = sc == -INFINITY ? 0.0f : expf(sc - mn);
-    m = mn;
-    __syncthreads();
-    l *= w;
-    acc[0] *= w;
-    acc[1] *= w;
-    const int tn = min(128, seen - t0);
-    for (int u = 0; u < tn; u++) {
-      const float p = ps[u];
-      if (p == 0.0f) continue;  // a hidden position's value is not touched
-      l += p;
-      const int tt = t0 + u;
+
+    float o[MT][NT][4] = {};
+    float m[NT][2], l[NT][2], f[NT][2];
+    int seen[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int d = tid + e * 128;
-        if (d >= hd) break;
-        float v;
-        if (tt < closed)
-          v = decode<KIND>(c.vc[(sh * c.cap + tt) * hd + d]) * c.vs[sh * (c.cap / kQ8Block) + tt / kQ8Block];
-        else
-          v = E::to(static_cast<const T*>(c.vt)[(sh * kQ8Block + tt - closed) * hd + d]);
-        acc[e] = fmaf(p, v, acc[e]);
+        const int x = n * 8 + 2 * cq + e;
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.0f;
+        f[n][e] = fac[x];
+        seen[n][e] = x0 + x >= R ? 0 : a.causal ? len - (s.nrow - 1 - (x0 + x) / G) : len;
+      }
+
+    int st = 0;
+    for (int t0 = t_first; t0 < t_end; t0 += S::UNIT) {
+      cp_wait<S::STAGES - 2>();
+      __syncwarp();  // the step has landed for every lane, and every lane is done with the last one
+      issue(t0 + (S::STAGES - 1) * S::UNIT, st == 0 ? S::STAGES - 1 : st - 1);
+      const unsigned char* kb = ring + st * S::STAGE;
+      const unsigned char* vb = kb + S::KBYTES;
+      const float* scl = reinterpret_cast<const float*>(kb + 2 * S::KBYTES);
+      st = st + 1 == S::STAGES ? 0 : st + 1;
+      // ---- scores of the step's blocks, in base 2
+      float sc[S::NG][NT][4];
+#pragma unroll
+      for (int g = 0; g < S::NG; g++) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) sc[g][n][e] = 0.0f;
+        uint32_t w0[KW < 4 ? KW : 4], w1[KW < 4 ? KW : 4];
+#pragma unroll
+        for (int k = 0; k < S::KS; k++) {
+          if constexpr (HDP >= 64) {
+            if (k % 4 == 0) {
+              *reinterpret_cast<uint4*>(w0) =
+                  *reinterpret_cast<const uint4*>(kb + qs_chunk<HDP>(g * 16 + r, k + cq));
+              *reinterpret_cast<uint4*>(w1) =
+                  *reinterpret_cast<const uint4*>(kb + qs_chunk<HDP>(g * 16 + r + 8, k + cq));
+            }
+          } else if (k == 0) {
+            *reinterpret_cast<uint2*>(w0) =
+                *reinterpret_cast<const uint2*>(kb + qs_chunk<HDP>(g * 16 + r, cq >> 1) + (cq & 1) * 8);
+            *reinterpret_cast<uint2*>(w1) =
+                *reinterpret_cast<const uint2*>(kb + qs_chunk<HDP>(g * 16 + r + 8, cq >> 1) + (cq & 1) * 8);
+          }
+          const uint32_t x = flip<KIND>(w0[k % 4]), y = flip<KIND>(w1[k % 4]);
+          const uint32_t af[4] = {halves<KIND, false>(x), halves<KIND, false>(y), halves<KIND, true>(x),
+                                  halves<KIND, true>(y)};
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+              const uint2 bf = qf[((k * NT + n) * QT + q) * 32 + lane];
+              mma16816(sc[g][n], af, bf.x, bf.y);
+            }
+        }
+        const float ks = scl[g];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) sc[g][n][e] *= ks * f[n][e & 1];
+      }
+      if (hide || t0 + S::TS > min(least, closed)) {
+#pragma unroll
+        for (int g = 0; g < S::NG; g++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int t = t0 + g * 16 + r + (e >> 1) * 8;
+            const bool hid = t >= closed || (hide && hide[t]);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+              if (hid || t >= seen[n][e & 1]) sc[g][n][e] = -INFINITY;
+          }
+      }
+      // ---- running maximum, weights (times 2^15) and their sum
+      uint32_t p[S::NG][NT][QT][2];
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float ref[2], al[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float mx = fmaxf(sc[0][n][e], sc[0][n][e + 2]);
+#pragma unroll
+          for (int g = 1; g < S::NG; g++) mx = fmaxf(mx, fmaxf(sc[g][n][e], sc[g][n][e + 2]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float mn = fmaxf(m[n][e], mx);
+          ref[e] = mn == -INFINITY ? 0.0f : mn;
+          al[e] = ex2(m[n][e] - ref[e]);
+          m[n][e] = mn;
+        }
+        if (__any_sync(0xffffffffu, !(al[0] == 1.0f && al[1] == 1.0f))) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) l[n][e] *= al[e];
+#pragma unroll
+          for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[j][n][e] *= al[e & 1];
+        }
+#pragma unroll
+        for (int g = 0; g < S::NG; g++)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {  // position r, then r + 8
+            const float p0 = ex2(sc[g][n][e] - ref[0]) * 32768.0f, p1 = ex2(sc[g][n][e + 1] - ref[1]) * 32768.0f;
+            l[n][0] += p0;
+            l[n][1] += p1;
+            const __half2 hi = __floats2half2_rn(p0, p1);
+            p[g][n][0][e >> 1] = transpose8(h2_bits(hi));
+            if constexpr (QT == 2) {
+              const float2 back = __half22float2(hi);
+              p[g][n][1][e >> 1] = transpose8(h2_bits(__floats2half2_rn(p0 - back.x, p1 - back.y)));
+            }
+          }
+      }
+      // ---- values
+#pragma unroll
+      for (int g = 0; g < S::NG; g++) {
+        const float vs = scl[S::NG + g];
+        const bool tiny = vs < 7.888609052210118e-31f;  // 2^-100: 2^-15 vs would lose bits
+        const float vs15 = tiny ? vs : vs * 3.0517578125e-05f;
+        constexpr int VW = HDP / 32;                 // words of a thread and position
+        constexpr int VL = VW < 4 ? VW : 4;          // of one load
+#pragma unroll
+        for (int w0 = 0; w0 < VW; w0 += VL) {
+          uint32_t w[4][VL];
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            const int t = g * 16 + 2 * cq + (q & 1) + (q >> 1) * 8;
+            if constexpr (HDP == 256)
+              *reinterpret_cast<uint4*>(w[q]) = *reinterpret_cast<const uint4*>(vb + qs_chunk<HDP>(t, 2 * r + w0 / 4));
+            else if constexpr (HDP == 128)
+              *reinterpret_cast<uint4*>(w[q]) = *reinterpret_cast<const uint4*>(vb + qs_chunk<HDP>(t, r));
+            else if constexpr (HDP == 64)
+              *reinterpret_cast<uint2*>(w[q]) =
+                  *reinterpret_cast<const uint2*>(vb + qs_chunk<HDP>(t, r >> 1) + (r & 1) * 8);
+            else
+              w[q][0] = *reinterpret_cast<const uint32_t*>(vb + qs_chunk<HDP>(t, r >> 2) + (r & 3) * 4);
+          }
+#pragma unroll
+          for (int v = 0; v < VL; v++) {
+            const uint32_t x0 = flip<KIND>(w[0][v]), x1 = flip<KIND>(w[1][v]);
+            const uint32_t y0 = flip<KIND>(w[2][v]), y1 = flip<KIND>(w[3][v]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {  // dims 4v + 2h, 4v + 2h + 1 of the thread's
+              const uint32_t x = __byte_perm(x0, x1, h ? 0x7362 : 0x5140);
+              const uint32_t y = __byte_perm(y0, y1, h ? 0x7362 : 0x5140);
+              const uint32_t af[4] = {halves<KIND, false>(x), halves<KIND, true>(x), halves<KIND, false>(y),
+                                      halves<KIND, true>(y)};
+              const int j = 2 * (w0 + v) + h;
+#pragma unroll
+              for (int n = 0; n < NT; n++) {
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int q = 0; q < QT; q++) mma16816(d, af, p[g][n][q][0], p[g][n][q][1]);
+                if (tiny) {
+#pragma unroll
+                  for (int e = 0; e < 4; e++) d[e] *= 3.0517578125e-05f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[j][n][e] = fmaf(d[e], vs15, o[j][n][e]);
+              }
+            }
+          }
+        }
       }
     }
+    cp_wait<0>();
+
+    // ---- the open block: position closed + warp, closed + warp + 8
+    if (rank == ns - 1) {
+      const T* kt = static_cast<const T*>(c.kt) + sh * kQ8Block * hd;
+      const T* vt = static_cast<const T*>(c.vt) + sh * kQ8Block * hd;
+      for (int t = closed + warp; t < min(len, most); t += kQsWarps) {
+        if (hide && hide[t]) continue;
+        const T* kr = kt + (size_t)(t - closed) * hd;
+        const T* vr = vt + (size_t)(t - closed) * hd + r * (HDP / 8);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          float dot = 0.0f;  // of row r, over the thread's dims
+#pragma unroll
+          for (int k = 0; k < S::KS; k++) {
+            const int d0 = HDP >= 64 ? (k / 4 * 4 + cq) * 16 + k % 4 * 4 : cq * 8 + k * 4;
+            float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int x = QT - 1; x >= 0; x--) {
+              const uint2 bf = qf[((k * NT + n) * QT + x) * 32 + lane];
+              const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&bf.x));
+              const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&bf.y));
+              q[0] += lo.x;
+              q[1] += lo.y;
+              q[2] += hi.x;
+              q[3] += hi.y;
+            }
+            if (d0 < hd) {
+#pragma unroll
+              for (int e = 0; e < 4; e++) dot = fmaf(q[e], E::to(kr[d0 + e]), dot);
+            }
+          }
+          dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+          dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+          dot *= fac[n * 8 + r];
+          float w[2], al[2];
+          bool on[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float x = __shfl_sync(0xffffffffu, dot, (2 * cq + e) * 4);
+            on[e] = t < seen[n][e];
+            const float mn = on[e] ? fmaxf(m[n][e], x) : m[n][e];
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            al[e] = ex2(m[n][e] - ref);
+            w[e] = on[e] ? ex2(x - ref) : 0.0f;
+            m[n][e] = mn;
+            l[n][e] = l[n][e] * al[e] + (r == 0 ? w[e] * 32768.0f : 0.0f);
+          }
+#pragma unroll
+          for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int d = 2 * j + (e >> 1);
+              const float v = r * (HDP / 8) + d < hd ? E::to(vr[d]) : 0.0f;
+              const float y = o[j][n][e] * al[e & 1];
+              o[j][n][e] = on[e & 1] ? fmaf(w[e & 1], v, y) : y;
+            }
+        }
+      }
+    }
+
+    // ---- merge of the warps, in order
+    __syncwarp();  // every lane is done with the ring
+    float* wo = reinterpret_cast<float*>(ring);  // [ROWS][ORow]
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float x = l[n][e];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        const int row = n * 8 + 2 * cq + e;
+        if (r == 0) {
+          wm[warp * ROWS + row] = m[n][e];
+          wl[warp * ROWS + row] = x;
+        }
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+          *reinterpret_cast<float2*>(wo + row * S::ORow + r * (HDP / 8) + 2 * j) =
+              make_float2(o[j][n][e], o[j][n][e + 2]);
+      }
     __syncthreads();
+    const int rows = min(ROWS, R - x0);
+    for (int x = tid; x < rows * HDP; x += kQsWarps * 32) {
+      const int row = x / HDP, d = x % HDP;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kQsWarps; w++) M = fmaxf(M, wm[w * ROWS + row]);
+      float L = 0.0f, O = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kQsWarps; w++) {
+        const float wt = part_weight(wm[w * ROWS + row], M);
+        const float* src = reinterpret_cast<const float*>(sm + (size_t)w * S::STAGES * S::STAGE);
+        // a warp whose maximum is -inf holds zeros, or NaN from a NaN score
+        const float lw = wl[w * ROWS + row];
+        L = lw == lw ? fmaf(wt, lw, L) : lw;
+        O = fmaf(wt, src[row * S::ORow + d], O);
+      }
+      res[row * S::ORow + d] = O;
+      if (d == 0) {
+        cm[row] = M;
+        cm[ROWS + row] = L;
+      }
+    }
+    // ---- merge of the splits, in order; the rows' dims are dealt out over the cluster
+    if (csize > 1) cluster_arrive_wait();
+    else __syncthreads();
+    {
+      const uint32_t res_u = smem_u32(res), cm_u = smem_u32(cm);
+      for (int x = rank * kQsWarps * 32 + tid; x < rows * HDP; x += csize * kQsWarps * 32) {
+        const int row = x / HDP, d = x % HDP;
+        if (d >= hd) continue;
+        float M = -INFINITY, L = 0.0f, O = 0.0f;
+        if (csize > 1) {
+          for (int q = 0; q < ns; q++) M = fmaxf(M, ld_peer(peer_addr(cm_u + row * 4, q)));
+#pragma unroll 4
+          for (int q = 0; q < ns; q++) {
+            const float wt = part_weight(ld_peer(peer_addr(cm_u + row * 4, q)), M);
+            const float lw = ld_peer(peer_addr(cm_u + (ROWS + row) * 4, q));
+            L = lw == lw ? fmaf(wt, lw, L) : lw;
+            O = fmaf(wt, ld_peer(peer_addr(res_u + (row * S::ORow + d) * 4, q)), O);
+          }
+        } else {
+          L = cm[ROWS + row];
+          O = res[row * S::ORow + d];
+        }
+        // O is sum p v, L is 2^15 sum p; nothing seen: L = 0
+        const float y = L == 0.0f ? 0.0f : O / (L * 3.0517578125e-05f);
+        out0[(int64_t)(s.row0 + (x0 + row) / G) * a.out.token + (int64_t)(kvh * G + (x0 + row) % G) * a.out.head + d] =
+            E::from(y);
+      }
+    }
+    if (csize > 1) cluster_arrive_wait();  // peers are done with this CTA's result
+    else __syncthreads();
   }
-  for (int e = 0; e < 2; e++)
-    if (tid + e * 128 < hd) out[tid + e * 128] = E::from(l > 0.0f || l != l ? acc[e] / l : 0.0f);
 }
 
 // ------------------------------------------------------------------- host
@@ -422,11 +902,56 @@ void q8_read(const Q8View& c, int n, const int* lens, const int* start, const in
   DEFER_CUDA(cudaGetLastError());
 }
 
+namespace {
+
+// Kernel attributes are set once per device.
+bool first_on_device(unsigned long long& mask) {
+  int dev = 0;
+  DEFER_CUDA(cudaGetDevice(&dev));
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (mask & bit) return false;
+  mask |= bit;
+  return true;
+}
+
+template <int TYPE, int KIND, int HDP, int NT>
+void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st) {
+  auto kern = k_q8_attend<TYPE, KIND, HDP, NT>;
+  constexpr size_t smem = qs_smem<HDP, NT, TYPE == kQ8F32 ? 2 : 1>();
+  static unsigned long long attr = 0;
+  if (first_on_device(attr)) {
+    DEFER_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    DEFER_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  }
+  const int64_t rows = (int64_t)std::max(b.max_q, 1) * (a.heads / c.kvh);
+  const int64_t tiles = std::min<int64_t>((rows + 8 * NT - 1) / (8 * NT), 65535 / c.kvh);
+  int cl = 1;  // a power of two that holds the splits of the longest sequence
+  while (cl < qs_splits<HDP>(a.max_len / kQ8Block * kQ8Block)) cl *= 2;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = cl;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(b.n * cl), (unsigned)(c.kvh * tiles), 1);
+  cfg.blockDim = dim3(kQsWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  DEFER_CUDA(cudaLaunchKernelEx(&cfg, kern, c, b, a, (int)tiles));
+}
+
+}  // namespace
+
 void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st) {
   if (b.n == 0 || b.tokens == 0) return;
-  const dim3 grid(b.tokens, a.heads);
+  const bool one = (int64_t)b.max_q * (a.heads / c.kvh) <= 8;
   dispatch(c, [&](auto type, auto kind) {
-    k_q8_attend<decltype(type)::value, decltype(kind)::value><<<grid, 128, 0, st>>>(c, b, a);
+    constexpr int TY = decltype(type)::value, KI = decltype(kind)::value;
+    if (c.hd <= 32) one ? attend_few<TY, KI, 32, 1>(c, b, a, st) : attend_few<TY, KI, 32, 2>(c, b, a, st);
+    else if (c.hd <= 64) one ? attend_few<TY, KI, 64, 1>(c, b, a, st) : attend_few<TY, KI, 64, 2>(c, b, a, st);
+    else if (c.hd <= 128) one ? attend_few<TY, KI, 128, 1>(c, b, a, st) : attend_few<TY, KI, 128, 2>(c, b, a, st);
+    else attend_few<TY, KI, 256, 1>(c, b, a, st);
   });
   DEFER_CUDA(cudaGetLastError());
 }
