@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // the last split, a token a warp, in fp32.
 constexpr int kQsWarps = 8;
 constexpr int kQsMaxSplits = 16;
+constexpr int kQsMinUnits = 2;  // units of a split, when there are as many
 
 template <int HDP>
 struct QsShape {
@@ -310,6 +311,7 @@ struct QsShape {
   static constexpr int STAGES = HDP == 256 ? 2 : 3;
   static constexpr int KBYTES = TS * HDP;
   static constexpr int STAGE = 2 * KBYTES + 2 * NG * 4 + (32 - 2 * NG * 4 % 32) % 32;  // codes, scales, pad
+  static constexpr int OPENV = STAGE / 32 * 16;            // where the open block's values start
   static constexpr int UNIT = kQsWarps * TS;               // positions of one step of the CTA
   static constexpr int ORow = HDP + 4;                     // floats of a result row
 };
@@ -325,8 +327,8 @@ constexpr size_t qs_smem() {
 // Splits of a sequence with `closed` positions in closed blocks.
 template <int HDP>
 __host__ __device__ __forceinline__ int qs_splits(int closed) {
-  const int units = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT;
-  return units < 1 ? 1 : units > kQsMaxSplits ? kQsMaxSplits : units;
+  const int n = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT / kQsMinUnits;
+  return n < 1 ? 1 : n > kQsMaxSplits ? kQsMaxSplits : n;
 }
 
 // Byte offset of 16-byte chunk `ch` of position `t` in a step's K or V. The
@@ -357,6 +359,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 of 16 bits across the warp
   uint32_t y;
@@ -414,6 +421,15 @@ __device__ __forceinline__ float ld_peer(uint32_t a) {
   return v;
 }
 
+__device__ __forceinline__ float4 ld_peer4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+
 // Weight of a partial result with maximum m under the total's maximum M.
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(m - M); }
 
@@ -436,11 +452,11 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
   const int csize = (int)cluster_size(), rank = (int)cluster_rank();
   const int i = blockIdx.x / csize;
   const int kvh = blockIdx.y / tiles;
+  int len = __ldg(a.lens + i);
   const Seq s = seq_of(b, c.slots, i);
   const int G = a.heads / c.kvh, R = s.nrow * G;
-  // every CTA of a cluster takes the same way out
   if (s.slot == kSeqSkip || R == 0) return;
-  const int len = s.slot == kSeqBad ? -1 : __ldg(a.lens + i);
+  if (s.slot == kSeqBad) len = -1;
   T* const out0 = static_cast<T*>(const_cast<void*>(a.out.p));
   if (len < 0 || len > c.cap) {
     if (b.status && tid == 0) atomicOr(b.status, (int)kQ8BadRange);
@@ -451,6 +467,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
   }
   const int hd = c.hd, closed = len & ~(kQ8Block - 1);
   const int ns = min(qs_splits<HDP>(closed), csize);
+  if (rank >= ns) return;  // cluster barriers wait for the CTAs that are left
   const size_t sh = (size_t)s.slot * c.kvh + kvh;
   const unsigned char* kc = c.kc + sh * c.cap * hd;
   const unsigned char* vc = c.vc + sh * c.cap * hd;
@@ -467,33 +484,54 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
     // positions that the tile's last row sees bound the work of the tile
     const int most = a.causal ? min(len, len - (s.nrow - 1 - jlast / G)) : len;
     const int least = a.causal ? len - (s.nrow - 1 - x0 / G) : len;  // the first row's
-    const int u0 = rank < ns ? (int)((int64_t)units * rank / ns) : 0;
-    const int u1 = rank < ns ? (int)((int64_t)units * (rank + 1) / ns) : 0;
+    const int u0 = (int)((int64_t)units * rank / ns), u1 = (int)((int64_t)units * (rank + 1) / ns);
     const int t_end = min(min(closed, most), u1 * S::UNIT);
     const int t_first = u0 * S::UNIT + warp * S::TS;
+    const int steps = t_end > t_first ? (t_end - t_first + S::UNIT - 1) / S::UNIT : 0;
+    // positions of the open block that the warp adds: closed + warp (+ 8)
+    const int t_open = rank == ns - 1 ? min(len, most) - closed - warp : 0;
+    const int n_open = t_open > kQsWarps ? 2 : t_open > 0 ? 1 : 0;
 
-    auto issue = [&](int t0, int st) {
-      if (t0 < t_end) {
-        const uint32_t base = ring_u + st * S::STAGE;
+    // Step `it` of the warp into ring slot `st`; the last one is the open block's.
+    const int lt = lane / S::CH, lch = lane % S::CH;  // the lane's position and chunk in a copy of 32 chunks
+    const unsigned char* kp = kc + ((size_t)t_first + lt) * hd + lch * 16;
+    const unsigned char* vp = vc + ((size_t)t_first + lt) * hd + lch * 16;
+    const bool lane_on = lch * 16 < hd;
+    auto issue = [&](int it, int st) {
+      const uint32_t base = ring_u + st * S::STAGE;
+      if (it < steps) {
+        const int t0 = t_first + it * S::UNIT;
 #pragma unroll
         for (int e = 0; e < S::TS * S::CH / 32; e++) {
-          const int x = e * 32 + lane, t = x / S::CH, ch = x % S::CH;
-          const bool on = t0 + t < closed && ch * 16 < hd;
-          const size_t o = on ? (size_t)(t0 + t) * hd + ch * 16 : 0;
-          const uint32_t d = base + qs_chunk<HDP>(t, ch);
-          cp16(d, kc + o, on);
-          cp16(d + S::KBYTES, vc + o, on);
+          const int t = e * (32 / S::CH) + lt;
+          // closed is a multiple of 16: only a step of several blocks can end before its last
+          const bool on = lane_on && (S::NG == 1 || t0 + t < closed);
+          const size_t o = on ? (size_t)(e * (32 / S::CH)) * hd : 0;
+          const uint32_t d = base + qs_chunk<HDP>(t, lch);
+          cp16(d, on ? kp + o : kc, on);
+          cp16(d + S::KBYTES, on ? vp + o : vc, on);
         }
+        kp += (size_t)S::UNIT * hd;
+        vp += (size_t)S::UNIT * hd;
         if (lane < 2 * S::NG) {
           const int g = lane % S::NG;
           const bool on = t0 + g * kQ8Block < closed;
           cp4(base + 2 * S::KBYTES + lane * 4, (lane < S::NG ? ksc : vsc) + (on ? t0 / kQ8Block + g : 0), on);
         }
+      } else if (it == steps && n_open) {
+        const int row = hd * (int)sizeof(T) / 16;  // chunks of a token
+        const uint4* k16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.kt) + (sh * kQ8Block + warp) * hd);
+        const uint4* v16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.vt) + (sh * kQ8Block + warp) * hd);
+        for (int x = lane; x < n_open * row; x += 32) {
+          const int y = x < row ? x : x + (kQsWarps - 1) * row;  // the second token is 8 rows on
+          cp16(base + x * 16, k16 + y, true);
+          cp16(base + S::OPENV + x * 16, v16 + y, true);
+        }
       }
       cp_commit();
     };
 #pragma unroll
-    for (int st = 0; st < S::STAGES - 1; st++) issue(t_first + st * S::UNIT, st);
+    for (int st = 0; st < S::STAGES - 1; st++) issue(st, st);
 
     // q rows of the tile as score operands: warp w takes rows w, w + 8
     for (int x = warp; x < ROWS; x += kQsWarps) {
@@ -550,10 +588,11 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
       }
 
     int st = 0;
-    for (int t0 = t_first; t0 < t_end; t0 += S::UNIT) {
+    for (int it = 0; it < steps; it++) {
+      const int t0 = t_first + it * S::UNIT;
       cp_wait<S::STAGES - 2>();
       __syncwarp();  // the step has landed for every lane, and every lane is done with the last one
-      issue(t0 + (S::STAGES - 1) * S::UNIT, st == 0 ? S::STAGES - 1 : st - 1);
+      issue(it + S::STAGES - 1, st == 0 ? S::STAGES - 1 : st - 1);
       const unsigned char* kb = ring + st * S::STAGE;
       const unsigned char* vb = kb + S::KBYTES;
       const float* scl = reinterpret_cast<const float*>(kb + 2 * S::KBYTES);
@@ -562,10 +601,6 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
       float sc[S::NG][NT][4];
 #pragma unroll
       for (int g = 0; g < S::NG; g++) {
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) sc[g][n][e] = 0.0f;
         uint32_t w0[KW < 4 ? KW : 4], w1[KW < 4 ? KW : 4];
 #pragma unroll
         for (int k = 0; k < S::KS; k++) {
@@ -590,7 +625,8 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
 #pragma unroll
             for (int q = 0; q < QT; q++) {
               const uint2 bf = qf[((k * NT + n) * QT + q) * 32 + lane];
-              mma16816(sc[g][n], af, bf.x, bf.y);
+              if (k == 0 && q == 0) mma16816_zero(sc[g][n], af, bf.x, bf.y);
+              else mma16816(sc[g][n], af, bf.x, bf.y);
             }
         }
         const float ks = scl[g];
@@ -654,9 +690,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
       // ---- values
 #pragma unroll
       for (int g = 0; g < S::NG; g++) {
-        const float vs = scl[S::NG + g];
-        const bool tiny = vs < 7.888609052210118e-31f;  // 2^-100: 2^-15 vs would lose bits
-        const float vs15 = tiny ? vs : vs * 3.0517578125e-05f;
+        const float vs15 = scl[S::NG + g] * 3.0517578125e-05f;
         constexpr int VW = HDP / 32;                 // words of a thread and position
         constexpr int VL = VW < 4 ? VW : 4;          // of one load
 #pragma unroll
@@ -688,13 +722,9 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
               const int j = 2 * (w0 + v) + h;
 #pragma unroll
               for (int n = 0; n < NT; n++) {
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int q = 0; q < QT; q++) mma16816(d, af, p[g][n][q][0], p[g][n][q][1]);
-                if (tiny) {
-#pragma unroll
-                  for (int e = 0; e < 4; e++) d[e] *= 3.0517578125e-05f;
-                }
+                float d[4];
+                mma16816_zero(d, af, p[g][n][0][0], p[g][n][0][1]);
+                if constexpr (QT == 2) mma16816(d, af, p[g][n][1][0], p[g][n][1][1]);
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[j][n][e] = fmaf(d[e], vs15, o[j][n][e]);
               }
@@ -704,15 +734,16 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
       }
     }
     cp_wait<0>();
+    __syncwarp();
 
-    // ---- the open block: position closed + warp, closed + warp + 8
-    if (rank == ns - 1) {
-      const T* kt = static_cast<const T*>(c.kt) + sh * kQ8Block * hd;
-      const T* vt = static_cast<const T*>(c.vt) + sh * kQ8Block * hd;
-      for (int t = closed + warp; t < min(len, most); t += kQsWarps) {
+    // ---- the open block
+    {
+      const T* kb = reinterpret_cast<const T*>(ring + st * S::STAGE);
+      const T* vb = reinterpret_cast<const T*>(ring + st * S::STAGE + S::OPENV) + r * (HDP / 8);
+      for (int y = 0; y < n_open; y++) {
+        const int t = closed + warp + y * kQsWarps;
         if (hide && hide[t]) continue;
-        const T* kr = kt + (size_t)(t - closed) * hd;
-        const T* vr = vt + (size_t)(t - closed) * hd + r * (HDP / 8);
+        const T *kr = kb + y * hd, *vr = vb + y * hd;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           float dot = 0.0f;  // of row r, over the thread's dims
@@ -786,22 +817,25 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
       }
     __syncthreads();
     const int rows = min(ROWS, R - x0);
-    for (int x = tid; x < rows * HDP; x += kQsWarps * 32) {
-      const int row = x / HDP, d = x % HDP;
+    for (int x = tid; x < rows * (HDP / 4); x += kQsWarps * 32) {
+      const int row = x / (HDP / 4), d = x % (HDP / 4) * 4;
       float M = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kQsWarps; w++) M = fmaxf(M, wm[w * ROWS + row]);
-      float L = 0.0f, O = 0.0f;
+      float L = 0.0f, O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < kQsWarps; w++) {
         const float wt = part_weight(wm[w * ROWS + row], M);
-        const float* src = reinterpret_cast<const float*>(sm + (size_t)w * S::STAGES * S::STAGE);
+        const float4 y = *reinterpret_cast<const float4*>(sm + (size_t)w * S::STAGES * S::STAGE +
+                                                          (row * S::ORow + d) * sizeof(float));
         // a warp whose maximum is -inf holds zeros, or NaN from a NaN score
-        const float lw = wl[w * ROWS + row];
-        L = lw == lw ? fmaf(wt, lw, L) : lw;
-        O = fmaf(wt, src[row * S::ORow + d], O);
+        L = fmaf(wt, wl[w * ROWS + row], L);
+        O[0] = fmaf(wt, y.x, O[0]);
+        O[1] = fmaf(wt, y.y, O[1]);
+        O[2] = fmaf(wt, y.z, O[2]);
+        O[3] = fmaf(wt, y.w, O[3]);
       }
-      res[row * S::ORow + d] = O;
+      *reinterpret_cast<float4*>(res + row * S::ORow + d) = make_float4(O[0], O[1], O[2], O[3]);
       if (d == 0) {
         cm[row] = M;
         cm[ROWS + row] = L;
@@ -812,27 +846,34 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
     else __syncthreads();
     {
       const uint32_t res_u = smem_u32(res), cm_u = smem_u32(cm);
-      for (int x = rank * kQsWarps * 32 + tid; x < rows * HDP; x += csize * kQsWarps * 32) {
-        const int row = x / HDP, d = x % HDP;
+      for (int x = rank * kQsWarps * 32 + tid; x < rows * (HDP / 4); x += ns * kQsWarps * 32) {
+        const int row = x / (HDP / 4), d = x % (HDP / 4) * 4;
         if (d >= hd) continue;
-        float M = -INFINITY, L = 0.0f, O = 0.0f;
-        if (csize > 1) {
+        float L, O[4];
+        if (ns > 1) {
+          float M = -INFINITY;
+#pragma unroll 4
           for (int q = 0; q < ns; q++) M = fmaxf(M, ld_peer(peer_addr(cm_u + row * 4, q)));
+          L = O[0] = O[1] = O[2] = O[3] = 0.0f;
 #pragma unroll 4
           for (int q = 0; q < ns; q++) {
             const float wt = part_weight(ld_peer(peer_addr(cm_u + row * 4, q)), M);
-            const float lw = ld_peer(peer_addr(cm_u + (ROWS + row) * 4, q));
-            L = lw == lw ? fmaf(wt, lw, L) : lw;
-            O = fmaf(wt, ld_peer(peer_addr(res_u + (row * S::ORow + d) * 4, q)), O);
+            const float4 y = ld_peer4(peer_addr(res_u + (row * S::ORow + d) * 4, q));
+            L = fmaf(wt, ld_peer(peer_addr(cm_u + (ROWS + row) * 4, q)), L);
+            O[0] = fmaf(wt, y.x, O[0]);
+            O[1] = fmaf(wt, y.y, O[1]);
+            O[2] = fmaf(wt, y.z, O[2]);
+            O[3] = fmaf(wt, y.w, O[3]);
           }
         } else {
           L = cm[ROWS + row];
-          O = res[row * S::ORow + d];
+#pragma unroll
+          for (int e = 0; e < 4; e++) O[e] = res[row * S::ORow + d + e];
         }
         // O is sum p v, L is 2^15 sum p; nothing seen: L = 0
-        const float y = L == 0.0f ? 0.0f : O / (L * 3.0517578125e-05f);
-        out0[(int64_t)(s.row0 + (x0 + row) / G) * a.out.token + (int64_t)(kvh * G + (x0 + row) % G) * a.out.head + d] =
-            E::from(y);
+        T* y = out0 + (int64_t)(s.row0 + (x0 + row) / G) * a.out.token + (int64_t)(kvh * G + (x0 + row) % G) * a.out.head + d;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = E::from(L == 0.0f ? 0.0f : O[e] / (L * 3.0517578125e-05f));
       }
     }
     if (csize > 1) cluster_arrive_wait();  // peers are done with this CTA's result
@@ -927,17 +968,21 @@ void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream
   const int64_t tiles = std::min<int64_t>((rows + 8 * NT - 1) / (8 * NT), 65535 / c.kvh);
   int cl = 1;  // a power of two that holds the splits of the longest sequence
   while (cl < qs_splits<HDP>(a.max_len / kQ8Block * kQ8Block)) cl *= 2;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = cl;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cl;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  // a cluster's CTAs on as many SMs as there are, not two on one: a single
+  // long sequence has fewer CTAs than the device has SMs
+  at[1].id = cudaLaunchAttributeClusterSchedulingPolicyPreference;
+  at[1].val.clusterSchedulingPolicyPreference = cudaClusterSchedulingPolicySpread;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(b.n * cl), (unsigned)(c.kvh * tiles), 1);
   cfg.blockDim = dim3(kQsWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
   DEFER_CUDA(cudaLaunchKernelEx(&cfg, kern, c, b, a, (int)tiles));
 }
 
