@@ -128,7 +128,8 @@ SIGNATURES = [
     ("defer_q8_read", ctypes.c_int, [vp, u32, vp, vp, vp, vp, u32, vp, ctypes.POINTER(i64), vp, ctypes.POINTER(i64),
                                      vp]),
     ("defer_q8_attend", ctypes.c_int, [vp, vp, vp, u32, u32, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.c_int32,
-                                       ctypes.c_float, vp]),
+                                       ctypes.c_float, vp, sz, vp]),
+    ("defer_q8_attend_workspace", ctypes.c_int, [vp, vp, u32, u32, c_szp]),
     ("defer_log_softmax_at", ctypes.c_double, [c_f32p, sz, sz]),
 ]
 

@@ -118,6 +118,14 @@ defer::Q8Batch q8_batch(const defer::Q8View& c, const defer_q8_batch* b) {
   return {(int)b->n, (int)b->tokens, (int)mq, b->q_start, b->slots, b->status};
 }
 
+void q8_heads(const defer::Q8View& c, uint32_t heads) {
+  q8_check(heads >= 1 && heads % (uint32_t)c.kvh == 0 && heads <= 16384, "heads must be a multiple of kv_heads");
+}
+
+int q8_most(const defer::Q8View& c, uint32_t max_len) {
+  return max_len ? (int)std::min<uint32_t>(max_len, (uint32_t)c.cap) : c.cap;
+}
+
 // Whether rows of `len` elements at strides (count, stride) overlap.
 bool q8_overlap(int64_t len, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
   std::vector<std::pair<int64_t, int64_t>> d;  // (stride, count)
@@ -730,14 +738,28 @@ int defer_q8_read(const defer_q8_cache* cache, uint32_t n, const int32_t* lens, 
   });
 }
 
-int defer_q8_attend(const defer_q8_cache* cache, const defer_q8_batch* batch, const int32_t* lens, uint32_t max_len,
-                    uint32_t heads, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
-                    int64_t out_token_stride, int64_t out_head_stride, const uint8_t* masked, int64_t mask_stride,
-                    int32_t causal, float scale, void* stream) {
+int defer_q8_attend_workspace(const defer_q8_cache* cache, const defer_q8_batch* batch, uint32_t max_len,
+                              uint32_t heads, size_t* bytes) {
   return guard([&] {
     const defer::Q8View c = q8_view(cache);
     const defer::Q8Batch b = q8_batch(c, batch);
-    q8_check(heads >= 1 && heads % (uint32_t)c.kvh == 0 && heads <= 16384, "heads must be a multiple of kv_heads");
+    need(bytes, "bytes");
+    q8_heads(c, heads);
+    defer::Q8Attend a{};
+    a.max_len = q8_most(c, max_len);
+    a.heads = (int)heads;
+    *bytes = defer::q8_attend_workspace(c, b, a);
+  });
+}
+
+int defer_q8_attend(const defer_q8_cache* cache, const defer_q8_batch* batch, const int32_t* lens, uint32_t max_len,
+                    uint32_t heads, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                    int64_t out_token_stride, int64_t out_head_stride, const uint8_t* masked, int64_t mask_stride,
+                    int32_t causal, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  return guard([&] {
+    const defer::Q8View c = q8_view(cache);
+    const defer::Q8Batch b = q8_batch(c, batch);
+    q8_heads(c, heads);
     q8_check(std::isfinite(scale), "scale must be finite");
     q8_check(!masked || mask_stride == 0 || mask_stride >= c.cap, "masked must have a byte for each of cap positions");
     if (b.n == 0 || b.tokens == 0) return;
@@ -745,12 +767,14 @@ int defer_q8_attend(const defer_q8_cache* cache, const defer_q8_batch* batch, co
     need(q, "q");
     need(out, "out");
     q8_check(!q8_overlap(c.hd, {{b.tokens, out_token_stride}, {heads, out_head_stride}}), "the output's rows overlap");
-    const int most = max_len ? (int)std::min<uint32_t>(max_len, (uint32_t)c.cap) : c.cap;
+    const defer::Q8Attend a{lens, q8_most(c, max_len), (int)heads, {q, q_token_stride, q_head_stride},
+                            {out, out_token_stride, out_head_stride}, masked, mask_stride, causal != 0, scale,
+                            static_cast<float*>(workspace)};
+    const size_t bytes = defer::q8_attend_workspace(c, b, a);
+    q8_check(bytes == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= bytes),
+             "the workspace is smaller than defer_q8_attend_workspace, or not 16-byte aligned");
     OnDevice on(cache->device);
-    defer::q8_attend(c, b,
-                     {lens, most, (int)heads, {q, q_token_stride, q_head_stride}, {out, out_token_stride, out_head_stride},
-                      masked, mask_stride, causal != 0, scale},
-                     static_cast<cudaStream_t>(stream));
+    defer::q8_attend(c, b, a, static_cast<cudaStream_t>(stream));
   });
 }
 

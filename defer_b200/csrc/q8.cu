@@ -280,48 +280,53 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // tensor cores (mma m16n8k16, fp32 sums). The other operand is made as exact
 // as the cache's type asks: a q row is scaled by a power of two so that its
 // largest element is in [2^14, 2^15) and held as one fp16 term (bf16 and fp16
-// rows: no bit lost) or two (fp32: 22 bits); P is kept times 2^15, so that
-// weights down to 2^-29 of the largest are full fp16 numbers, and held the
-// same way. Products of one block of 16 positions are summed by the tensor
-// core from zero and added to the running sums in fp32 registers: long chains
-// inside the tensor core lose bits. Softmax: running maximum and sum per warp
-// in base 2; warps, then splits, are merged in order.
+// rows: no bit lost) or two (fp32: 22 bits). The weights take the value scale
+// with them, P' = 2^(x + log2 s_V - m) with the running maximum m taken over
+// x + floor(log2 s_V) (x: score in base 2): times 2^14 they use fp16's whole
+// range, relative to the largest contribution to the output whatever the
+// scales of the other blocks are (one term, or two for fp32). The sum of the
+// weights themselves, 2^(x - m), stays in fp32. fp32 caches add the products
+// of each step to fp32 registers (a long chain of sums inside the tensor core
+// would lose bits that a 16-bit result does not have). Softmax: running
+// maximum and sum per warp; warps, then splits, are merged in order.
 //
 // Work. The positions of the closed blocks are cut into units of 8 warp
-// steps, the units into splits, one CTA each, the splits of a (sequence, key
+// steps, the units into splits, one CTA each, 8 splits of a (sequence, key
 // head, row tile) forming a cluster: partial results travel through
-// distributed shared memory, so the call needs no workspace and no second
-// launch. The number of splits follows from the sequence's length alone, so
-// its result does not depend on the batch it runs in. Each warp streams its
-// own steps (4 KB of K and V) through a ring of its own with 16-byte
-// asynchronous copies, without any barrier; chunks are swizzled so that both
-// the row-wise reads of K and the column-wise reads of V are free of bank
-// conflicts. The open block (fp32 or 16-bit tokens) is added at the end by
-// the last split, a token a warp, in fp32.
+// distributed shared memory, and up to 8 splits need no workspace and no
+// second launch. The clusters of longer sequences leave theirs in the
+// workspace, for k_q8_merge. The number of splits follows from the sequence's
+// length alone, so its result does not depend on the batch it runs in. A warp loads its steps
+// (4 KB of K and V) straight into the registers of the matrix instruction:
+// the order of the dims inside the score product, and of the dims of the
+// output, is free, so a thread takes 16 neighbouring bytes of a position
+// wherever it can, and nothing of the stream passes through shared memory.
+// K is loaded again as soon as its scores are done and V as soon as its
+// products are, and every lane asks for one 128-byte line of a step further
+// on to be brought into L2, which keeps enough bytes on their way. The open
+// block (fp32 or 16-bit tokens) is added at the end by the last split, a
+// token a warp, in fp32.
 constexpr int kQsWarps = 8;
-constexpr int kQsMaxSplits = 16;
-constexpr int kQsMinUnits = 2;  // units of a split, when there are as many
+constexpr int kQsCluster = 8;     // splits of a cluster
+constexpr int kQsMaxSplits = 64;  // of a sequence
+constexpr int kQsMinUnits = 8;    // units of a split, when there are as many
 
 template <int HDP>
 struct QsShape {
   static constexpr int TS = HDP >= 128 ? 16 : 2048 / HDP;  // positions of a warp step
   static constexpr int NG = TS / kQ8Block;                 // blocks of a step
-  static constexpr int CH = HDP / 16;                      // 16-byte chunks of a row
   static constexpr int KS = HDP / 16;                      // k steps of the score product
-  static constexpr int STAGES = HDP == 256 ? 2 : 3;
-  static constexpr int KBYTES = TS * HDP;
-  static constexpr int STAGE = 2 * KBYTES + 2 * NG * 4 + (32 - 2 * NG * 4 % 32) % 32;  // codes, scales, pad
-  static constexpr int OPENV = STAGE / 32 * 16;            // where the open block's values start
   static constexpr int UNIT = kQsWarps * TS;               // positions of one step of the CTA
   static constexpr int ORow = HDP + 4;                     // floats of a result row
+  static constexpr int KW = HDP / 16, VW = HDP / 32;       // words of K (V) a thread holds of one position
+  static constexpr int AHEAD = 4;                          // steps that L2 is asked to bring in advance
 };
 template <int HDP, int NT, int QT>
 constexpr size_t qs_smem() {
   using S = QsShape<HDP>;
-  return (size_t)kQsWarps * S::STAGES * S::STAGE          // rings (later the warps' results)
-         + (size_t)S::KS * NT * QT * 32 * 8               // q
-         + (size_t)(8 * NT) * S::ORow * 4                 // the CTA's result
-         + (size_t)(8 * NT) * (3 + 2 * kQsWarps) * 4;     // row factors, m and l of the CTA and of the warps
+  return (size_t)(kQsWarps + 1) * 8 * NT * S::ORow * 4     // results of the warps and of the CTA
+         + (size_t)S::KS * NT * QT * 32 * 8                // q
+         + (size_t)(8 * NT) * (3 + 2 * kQsWarps) * 4;      // row factors, m and l of the CTA and of the warps
 }
 
 // Splits of a sequence with `closed` positions in closed blocks.
@@ -331,29 +336,36 @@ __host__ __device__ __forceinline__ int qs_splits(int closed) {
   return n < 1 ? 1 : n > kQsMaxSplits ? kQsMaxSplits : n;
 }
 
-// Byte offset of 16-byte chunk `ch` of position `t` in a step's K or V. The
-// exclusive-or keeps a 128-byte phase of both access patterns on 32 banks: K
-// is read by 8 threads as 2 neighbouring rows x 4 chunks (or whole rows), V as
-// rows 2c (or 2c + 1), c = 0..3, x neighbouring chunks.
-template <int HDP>
-__device__ __forceinline__ int qs_chunk(int t, int ch) {
-  if constexpr (HDP == 256) return t * 256 + ((ch ^ ((t >> 1 & 1) | (((t >> 2) ^ t) & 1) << 2)) << 4);
-  else if constexpr (HDP == 128) return t * 128 + ((ch ^ ((t & 6) ^ (t & 1) << 2)) << 4);
-  else if constexpr (HDP == 64) return (t >> 1) * 128 + ((((t & 1) * 4 + ch) ^ ((t >> 1 & 3) * 2)) << 4);
-  else return (t >> 2) * 128 + ((((t & 3) * 2 + ch) ^ ((t >> 2 & 1) * 2)) << 4);
-}
+// Position (of 8) that row r of the score product stands for: the positions of
+// threads c = 0..3 in the value product, rows 2c and 2c + 1, are then
+// neighbours.
+__device__ __forceinline__ int qs_row(int r) { return (r >> 1) + (r & 1) * 4; }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+__device__ __forceinline__ void cp_join() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// W = 1, 2 or 4 words, past L1; where `on` is 0 the words stay as they are.
+template <int W>
+__device__ __forceinline__ void ld_words(uint32_t* w, const unsigned char* p, int on) {
+  if constexpr (W == 4)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\t"
+        "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+        : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])
+        : "l"(p), "r"(on));
+  else if constexpr (W == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\t@p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n\t}"
+        : "+r"(w[0]), "+r"(w[1])
+        : "l"(p), "r"(on));
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t@p ld.global.nc.L1::no_allocate.u32 %0, [%1];\n\t}"
+                 : "+r"(w[0])
+                 : "l"(p), "r"(on));
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -373,7 +385,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 of 16 bit
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -430,28 +442,40 @@ __device__ __forceinline__ float4 ld_peer4(uint32_t a) {
   return v;
 }
 
+// Exponent of a value scale (floor of its base-2 logarithm), from -100 up.
+__device__ __forceinline__ float scale_exponent(float v) {
+  return (float)max((__float_as_int(v) >> 23) - 127, -100);
+}
+
 // Weight of a partial result with maximum m under the total's maximum M.
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(m - M); }
 
-template <int TYPE, int KIND, int HDP, int NT>
-__global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
+// EXACT: head_dim is HDP; else HDP is the next instantiated size and the
+// dims behind head_dim are zeros that are not read.
+template <int TYPE, int KIND, int HDP, int NT, bool EXACT>
+__global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 1 : 2)
     k_q8_attend(const __grid_constant__ Q8View c, const __grid_constant__ Q8Batch b, const __grid_constant__ Q8Attend a,
-                int tiles) {
+                int tiles, int groups) {
   using S = QsShape<HDP>;
   using E = Elem<TYPE>;
   using T = typename E::T;
-  constexpr int QT = TYPE == kQ8F32 ? 2 : 1, ROWS = 8 * NT, MT = HDP / 16, KW = HDP / 16;
+  constexpr int QT = TYPE == kQ8F32 ? 2 : 1, ROWS = 8 * NT, MT = HDP / 16;
+  constexpr int WO = ROWS * S::ORow;  // floats of a warp's result; before that, its two tokens of the open block
+  constexpr int KL = S::KW < 4 ? S::KW : 4, VL = S::VW < 4 ? S::VW : 4;  // words of one load
+  static_assert(WO * 4 >= 4 * HDP * (int)sizeof(T), "the open block's tokens fit");
   extern __shared__ __align__(128) unsigned char sm[];
-  uint2* qf = reinterpret_cast<uint2*>(sm + (size_t)kQsWarps * S::STAGES * S::STAGE);
-  float* res = reinterpret_cast<float*>(qf + S::KS * NT * QT * 32);  // [ROWS][ORow]
-  float* fac = res + ROWS * S::ORow;                                  // [ROWS] row factors
+  float* wo_all = reinterpret_cast<float*>(sm);
+  float* res = wo_all + kQsWarps * WO;                  // [ROWS][ORow]
+  uint2* qf = reinterpret_cast<uint2*>(res + WO);
+  float* fac = reinterpret_cast<float*>(qf + S::KS * NT * QT * 32);  // [ROWS] row factors
   float* cm = fac + ROWS;                                             // [ROWS] the CTA's m, then l
   float* wm = cm + 2 * ROWS;                                          // [warps][ROWS] m, then [warps][ROWS] l
   float* wl = wm + kQsWarps * ROWS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, cq = lane & 3;
   const int csize = (int)cluster_size(), rank = (int)cluster_rank();
-  const int i = blockIdx.x / csize;
-  const int kvh = blockIdx.y / tiles;
+  const int i = (int)((unsigned)blockIdx.x / (unsigned)(csize * groups));
+  const int group = (int)((unsigned)blockIdx.x / (unsigned)csize) - i * groups;
+  const int kvh = (int)((unsigned)blockIdx.y / (unsigned)tiles);
   int len = __ldg(a.lens + i);
   const Seq s = seq_of(b, c.slots, i);
   const int G = a.heads / c.kvh, R = s.nrow * G;
@@ -460,13 +484,14 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
   T* const out0 = static_cast<T*>(const_cast<void*>(a.out.p));
   if (len < 0 || len > c.cap) {
     if (b.status && tid == 0) atomicOr(b.status, (int)kQ8BadRange);
-    for (int x = (blockIdx.y - kvh * tiles) * csize + rank; x < R; x += tiles * csize)
+    for (int x = ((blockIdx.y - kvh * tiles) * groups + group) * csize + rank; x < R; x += tiles * groups * csize)
       for (int d = tid; d < c.hd; d += kQsWarps * 32)
         out0[(int64_t)(s.row0 + x / G) * a.out.token + (int64_t)(kvh * G + x % G) * a.out.head + d] = E::from(NAN);
     return;
   }
-  const int hd = c.hd, closed = len & ~(kQ8Block - 1);
-  const int ns = min(qs_splits<HDP>(closed), csize);
+  const int hd = EXACT ? HDP : c.hd, closed = len & ~(kQ8Block - 1);
+  const int splits = min(qs_splits<HDP>(closed), groups * csize);
+  const int split = group * kQsCluster + rank, ns = min(splits - group * kQsCluster, csize);  // ns: of the cluster
   if (rank >= ns) return;  // cluster barriers wait for the CTAs that are left
   const size_t sh = (size_t)s.slot * c.kvh + kvh;
   const unsigned char* kc = c.kc + sh * c.cap * hd;
@@ -474,8 +499,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
   const float* ksc = c.ks + sh * (c.cap / kQ8Block);
   const float* vsc = c.vs + sh * (c.cap / kQ8Block);
   const unsigned char* hide = a.masked ? a.masked + (int64_t)i * a.mask_stride : nullptr;
-  unsigned char* ring = sm + (size_t)warp * S::STAGES * S::STAGE;
-  const uint32_t ring_u = smem_u32(ring);
+  float* wo = wo_all + warp * WO;
   const int units = (closed + S::UNIT - 1) / S::UNIT;
 
   for (int tile = blockIdx.y - kvh * tiles; tile * ROWS < R; tile += tiles) {
@@ -484,54 +508,88 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
     // positions that the tile's last row sees bound the work of the tile
     const int most = a.causal ? min(len, len - (s.nrow - 1 - jlast / G)) : len;
     const int least = a.causal ? len - (s.nrow - 1 - x0 / G) : len;  // the first row's
-    const int u0 = (int)((int64_t)units * rank / ns), u1 = (int)((int64_t)units * (rank + 1) / ns);
+    const int u0 = (int)((unsigned)(units * split) / (unsigned)splits);
+    const int u1 = (int)((unsigned)(units * (split + 1)) / (unsigned)splits);
     const int t_end = min(min(closed, most), u1 * S::UNIT);
     const int t_first = u0 * S::UNIT + warp * S::TS;
     const int steps = t_end > t_first ? (t_end - t_first + S::UNIT - 1) / S::UNIT : 0;
     // positions of the open block that the warp adds: closed + warp (+ 8)
-    const int t_open = rank == ns - 1 ? min(len, most) - closed - warp : 0;
+    const int t_open = split == splits - 1 ? min(len, most) - closed - warp : 0;
     const int n_open = t_open > kQsWarps ? 2 : t_open > 0 ? 1 : 0;
 
-    // Step `it` of the warp into ring slot `st`; the last one is the open block's.
-    const int lt = lane / S::CH, lch = lane % S::CH;  // the lane's position and chunk in a copy of 32 chunks
-    const unsigned char* kp = kc + ((size_t)t_first + lt) * hd + lch * 16;
-    const unsigned char* vp = vc + ((size_t)t_first + lt) * hd + lch * 16;
-    const bool lane_on = lch * 16 < hd;
-    auto issue = [&](int it, int st) {
-      const uint32_t base = ring_u + st * S::STAGE;
-      if (it < steps) {
-        const int t0 = t_first + it * S::UNIT;
+    // this thread's words of a step: K of rows r and r + 8, V of 4 positions, of each block
+    uint32_t kw[S::NG][2][S::KW] = {}, vw[S::NG][4][S::VW] = {};
+    float ks[S::NG] = {}, vs[S::NG] = {};
+    const unsigned char* kp = kc + (size_t)(t_first + qs_row(r)) * hd + cq * (HDP >= 64 ? 16 : 8);
+    const unsigned char* vp = vc + (size_t)(t_first + cq) * hd + r * (HDP / 8);
+    const float *ksp = ksc + t_first / kQ8Block, *vsp = vsc + t_first / kQ8Block;
+    // Loads of step `it`; nothing changes when there is none. closed is a
+    // multiple of 16: a step of several blocks can end before its last one,
+    // whose words are then an earlier step's and whose positions are hidden.
+    auto load_k = [&](int it) {
+      const int t0 = t_first + it * S::UNIT;
 #pragma unroll
-        for (int e = 0; e < S::TS * S::CH / 32; e++) {
-          const int t = e * (32 / S::CH) + lt;
-          // closed is a multiple of 16: only a step of several blocks can end before its last
-          const bool on = lane_on && (S::NG == 1 || t0 + t < closed);
-          const size_t o = on ? (size_t)(e * (32 / S::CH)) * hd : 0;
-          const uint32_t d = base + qs_chunk<HDP>(t, lch);
-          cp16(d, on ? kp + o : kc, on);
-          cp16(d + S::KBYTES, on ? vp + o : vc, on);
-        }
-        kp += (size_t)S::UNIT * hd;
-        vp += (size_t)S::UNIT * hd;
-        if (lane < 2 * S::NG) {
-          const int g = lane % S::NG;
-          const bool on = t0 + g * kQ8Block < closed;
-          cp4(base + 2 * S::KBYTES + lane * 4, (lane < S::NG ? ksc : vsc) + (on ? t0 / kQ8Block + g : 0), on);
-        }
-      } else if (it == steps && n_open) {
-        const int row = hd * (int)sizeof(T) / 16;  // chunks of a token
-        const uint4* k16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.kt) + (sh * kQ8Block + warp) * hd);
-        const uint4* v16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.vt) + (sh * kQ8Block + warp) * hd);
-        for (int x = lane; x < n_open * row; x += 32) {
-          const int y = x < row ? x : x + (kQsWarps - 1) * row;  // the second token is 8 rows on
-          cp16(base + x * 16, k16 + y, true);
-          cp16(base + S::OPENV + x * 16, v16 + y, true);
-        }
+      for (int g = 0; g < S::NG; g++) {
+        const int on = S::NG == 1 ? it < steps : t0 + g * kQ8Block < t_end;
+        if (on) ks[g] = __ldg(ksp + g);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int w = 0; w < S::KW; w += KL)
+            ld_words<KL>(kw[g][h] + w, kp + (size_t)(g * 16 + h * 8) * hd + w * 16,
+                         on && (EXACT || (w / 4 * 4 + cq) * (HDP >= 64 ? 16 : 8) < hd));
       }
-      cp_commit();
+      kp += (size_t)S::UNIT * hd;
+      ksp += S::UNIT / kQ8Block;
     };
+    auto load_v = [&](int it) {
+      const int t0 = t_first + it * S::UNIT;
 #pragma unroll
-    for (int st = 0; st < S::STAGES - 1; st++) issue(st, st);
+      for (int g = 0; g < S::NG; g++) {
+        const int on = S::NG == 1 ? it < steps : t0 + g * kQ8Block < t_end;
+        if (on) vs[g] = __ldg(vsp + g);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+          for (int w = 0; w < S::VW; w += VL)
+            ld_words<VL>(vw[g][q] + w, vp + (size_t)(g * 16 + (q & 1) * 4 + (q >> 1) * 8) * hd + w * 4,
+                         on && (EXACT || r * (HDP / 8) + w * 4 < hd));
+      }
+      vp += (size_t)S::UNIT * hd;
+      vsp += S::UNIT / kQ8Block;
+    };
+    // The lines of step `it` towards L2, half the lanes K, half V; `it` goes up
+    // by one a call. The last lines of a step of several blocks, or of
+    // shorter rows, may lie behind the last block: those are left out.
+    const int line = (lane & 15) * (S::TS * HDP / 16);
+    const unsigned char* pf = (lane < 16 ? kc : vc) + (size_t)(t_first + S::UNIT) * hd + line;
+    auto ahead = [&](int it) {
+      bool on = it < steps, on2 = on;
+      if constexpr (!EXACT || S::NG > 1) {
+        const int64_t left = (int64_t)(t_end - t_first - it * S::UNIT) * hd;
+        on = line < left;
+        on2 = line + 128 < left;
+      }
+      if (on) asm volatile("prefetch.global.L2 [%0];" ::"l"(pf));
+      if constexpr (HDP == 256) {
+        if (on2) asm volatile("prefetch.global.L2 [%0];" ::"l"(pf + 128));
+      }
+      pf += (size_t)S::UNIT * hd;
+    };
+    load_k(0);
+    load_v(0);
+#pragma unroll
+    for (int it = 1; it < S::AHEAD; it++) ahead(it);
+    if (n_open) {
+      const int row = hd * (int)sizeof(T) / 16;  // 16-byte chunks of a token
+      const uint4* k16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.kt) + (sh * kQ8Block + warp) * hd);
+      const uint4* v16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.vt) + (sh * kQ8Block + warp) * hd);
+      for (int x = lane; x < n_open * row; x += 32) {
+        const int y = x < row ? x : x + (kQsWarps - 1) * row;  // the second token is 8 rows on
+        cp16(smem_u32(wo) + x * 16, k16 + y);
+        cp16(smem_u32(wo) + (2 * row + x) * 16, v16 + y);
+      }
+    }
 
     // q rows of the tile as score operands: warp w takes rows w, w + 8
     for (int x = warp; x < ROWS; x += kQsWarps) {
@@ -546,15 +604,13 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
         mx = fmaxf(mx, fabsf(v[e]));
       }
       mx = warp_max_all(mx);
-      // up = 2^(14 - exponent of mx); a zero, infinite or NaN row is not scaled
-      int ex = 0;
-      if (mx > 0.0f && mx <= FLT_MAX) {
-        frexpf(mx, &ex);  // mx in [2^(ex - 1), 2^ex)
-        ex = 15 - ex;
-      }
-      // the power is applied in two steps: 2^ex itself may exceed fp32's range
-      const float up0 = ldexpf(1.0f, ex / 2), up1 = ldexpf(1.0f, ex - ex / 2);
-      if (lane == 0) fac[x] = a.scale * 1.4426950408889634f / up0 / up1;
+      // q times 2^up is in [2^14, 2^15) at its largest (less for subnormal
+      // rows); a zero, infinite or NaN row is not scaled. The power is
+      // applied in two steps: 2^up itself may exceed fp32's range.
+      const int up = mx > 0.0f && mx <= FLT_MAX ? 141 - (__float_as_int(mx) >> 23) : 0;  // -113 .. 141
+      const float up0 = __int_as_float((127 + up / 2) << 23), up1 = __int_as_float((127 + up - up / 2) << 23);
+      if (lane == 0)
+        fac[x] = a.scale * 1.4426950408889634f * __int_as_float((127 - up / 2) << 23) * __int_as_float((127 - up + up / 2) << 23);
 #pragma unroll
       for (int e = 0; e < HDP / 32; e++) {
         const int d = e * 32 + lane;
@@ -587,37 +643,17 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
         seen[n][e] = x0 + x >= R ? 0 : a.causal ? len - (s.nrow - 1 - (x0 + x) / G) : len;
       }
 
-    int st = 0;
     for (int it = 0; it < steps; it++) {
       const int t0 = t_first + it * S::UNIT;
-      cp_wait<S::STAGES - 2>();
-      __syncwarp();  // the step has landed for every lane, and every lane is done with the last one
-      issue(it + S::STAGES - 1, st == 0 ? S::STAGES - 1 : st - 1);
-      const unsigned char* kb = ring + st * S::STAGE;
-      const unsigned char* vb = kb + S::KBYTES;
-      const float* scl = reinterpret_cast<const float*>(kb + 2 * S::KBYTES);
-      st = st + 1 == S::STAGES ? 0 : st + 1;
+      ahead(it + S::AHEAD);
       // ---- scores of the step's blocks, in base 2
       float sc[S::NG][NT][4];
 #pragma unroll
       for (int g = 0; g < S::NG; g++) {
-        uint32_t w0[KW < 4 ? KW : 4], w1[KW < 4 ? KW : 4];
+        float s2[NT][4];
 #pragma unroll
         for (int k = 0; k < S::KS; k++) {
-          if constexpr (HDP >= 64) {
-            if (k % 4 == 0) {
-              *reinterpret_cast<uint4*>(w0) =
-                  *reinterpret_cast<const uint4*>(kb + qs_chunk<HDP>(g * 16 + r, k + cq));
-              *reinterpret_cast<uint4*>(w1) =
-                  *reinterpret_cast<const uint4*>(kb + qs_chunk<HDP>(g * 16 + r + 8, k + cq));
-            }
-          } else if (k == 0) {
-            *reinterpret_cast<uint2*>(w0) =
-                *reinterpret_cast<const uint2*>(kb + qs_chunk<HDP>(g * 16 + r, cq >> 1) + (cq & 1) * 8);
-            *reinterpret_cast<uint2*>(w1) =
-                *reinterpret_cast<const uint2*>(kb + qs_chunk<HDP>(g * 16 + r + 8, cq >> 1) + (cq & 1) * 8);
-          }
-          const uint32_t x = flip<KIND>(w0[k % 4]), y = flip<KIND>(w1[k % 4]);
+          const uint32_t x = flip<KIND>(kw[g][0][k]), y = flip<KIND>(kw[g][1][k]);
           const uint32_t af[4] = {halves<KIND, false>(x), halves<KIND, false>(y), halves<KIND, true>(x),
                                   halves<KIND, true>(y)};
 #pragma unroll
@@ -625,38 +661,43 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
 #pragma unroll
             for (int q = 0; q < QT; q++) {
               const uint2 bf = qf[((k * NT + n) * QT + q) * 32 + lane];
+              // two chains: each product waits for the one before it
               if (k == 0 && q == 0) mma16816_zero(sc[g][n], af, bf.x, bf.y);
-              else mma16816(sc[g][n], af, bf.x, bf.y);
+              else if (k == 1 && q == 0) mma16816_zero(s2[n], af, bf.x, bf.y);
+              else mma16816(k & 1 ? s2[n] : sc[g][n], af, bf.x, bf.y);
             }
         }
-        const float ks = scl[g];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) sc[g][n][e] *= ks * f[n][e & 1];
+          for (int e = 0; e < 4; e++) sc[g][n][e] = (sc[g][n][e] + s2[n][e]) * (ks[g] * f[n][e & 1]);
       }
+      load_k(it + 1);
       if (hide || t0 + S::TS > min(least, closed)) {
 #pragma unroll
         for (int g = 0; g < S::NG; g++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const int t = t0 + g * 16 + r + (e >> 1) * 8;
+            const int t = t0 + g * 16 + qs_row(r) + (e >> 1) * 8;
             const bool hid = t >= closed || (hide && hide[t]);
 #pragma unroll
             for (int n = 0; n < NT; n++)
               if (hid || t >= seen[n][e & 1]) sc[g][n][e] = -INFINITY;
           }
       }
-      // ---- running maximum, weights (times 2^15) and their sum
+      // ---- running maximum of weight times value scale, weights, their sum
       uint32_t p[S::NG][NT][QT][2];
+      float lam[S::NG];
+#pragma unroll
+      for (int g = 0; g < S::NG; g++) lam[g] = scale_exponent(vs[g]);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         float ref[2], al[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          float mx = fmaxf(sc[0][n][e], sc[0][n][e + 2]);
+          float mx = fmaxf(sc[0][n][e], sc[0][n][e + 2]) + lam[0];
 #pragma unroll
-          for (int g = 1; g < S::NG; g++) mx = fmaxf(mx, fmaxf(sc[g][n][e], sc[g][n][e + 2]));
+          for (int g = 1; g < S::NG; g++) mx = fmaxf(mx, fmaxf(sc[g][n][e], sc[g][n][e + 2]) + lam[g]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           const float mn = fmaxf(m[n][e], mx);
@@ -675,10 +716,12 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
 #pragma unroll
         for (int g = 0; g < S::NG; g++)
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {  // position r, then r + 8
-            const float p0 = ex2(sc[g][n][e] - ref[0]) * 32768.0f, p1 = ex2(sc[g][n][e + 1] - ref[1]) * 32768.0f;
+          for (int e = 0; e < 4; e += 2) {  // rows r, then r + 8
+            float p0 = ex2(sc[g][n][e] - ref[0]), p1 = ex2(sc[g][n][e + 1] - ref[1]);
             l[n][0] += p0;
             l[n][1] += p1;
+            p0 = p0 * vs[g] * 16384.0f;  // in this order: the scale of hidden positions may be near the largest number
+            p1 = p1 * vs[g] * 16384.0f;
             const __half2 hi = __floats2half2_rn(p0, p1);
             p[g][n][0][e >> 1] = transpose8(h2_bits(hi));
             if constexpr (QT == 2) {
@@ -690,60 +733,50 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
       // ---- values
 #pragma unroll
       for (int g = 0; g < S::NG; g++) {
-        const float vs15 = scl[S::NG + g] * 3.0517578125e-05f;
-        constexpr int VW = HDP / 32;                 // words of a thread and position
-        constexpr int VL = VW < 4 ? VW : 4;          // of one load
 #pragma unroll
-        for (int w0 = 0; w0 < VW; w0 += VL) {
-          uint32_t w[4][VL];
+        for (int v = 0; v < S::VW; v++) {
+          const uint32_t x0 = flip<KIND>(vw[g][0][v]), x1 = flip<KIND>(vw[g][1][v]);
+          const uint32_t y0 = flip<KIND>(vw[g][2][v]), y1 = flip<KIND>(vw[g][3][v]);
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            const int t = g * 16 + 2 * cq + (q & 1) + (q >> 1) * 8;
-            if constexpr (HDP == 256)
-              *reinterpret_cast<uint4*>(w[q]) = *reinterpret_cast<const uint4*>(vb + qs_chunk<HDP>(t, 2 * r + w0 / 4));
-            else if constexpr (HDP == 128)
-              *reinterpret_cast<uint4*>(w[q]) = *reinterpret_cast<const uint4*>(vb + qs_chunk<HDP>(t, r));
-            else if constexpr (HDP == 64)
-              *reinterpret_cast<uint2*>(w[q]) =
-                  *reinterpret_cast<const uint2*>(vb + qs_chunk<HDP>(t, r >> 1) + (r & 1) * 8);
-            else
-              w[q][0] = *reinterpret_cast<const uint32_t*>(vb + qs_chunk<HDP>(t, r >> 2) + (r & 3) * 4);
-          }
+          for (int h = 0; h < 2; h++) {  // dims 4v + 2h, 4v + 2h + 1 of the thread's
+            const uint32_t x = __byte_perm(x0, x1, h ? 0x7362 : 0x5140);
+            const uint32_t y = __byte_perm(y0, y1, h ? 0x7362 : 0x5140);
+            const uint32_t af[4] = {halves<KIND, false>(x), halves<KIND, true>(x), halves<KIND, false>(y),
+                                    halves<KIND, true>(y)};
+            const int j = 2 * v + h;
 #pragma unroll
-          for (int v = 0; v < VL; v++) {
-            const uint32_t x0 = flip<KIND>(w[0][v]), x1 = flip<KIND>(w[1][v]);
-            const uint32_t y0 = flip<KIND>(w[2][v]), y1 = flip<KIND>(w[3][v]);
-#pragma unroll
-            for (int h = 0; h < 2; h++) {  // dims 4v + 2h, 4v + 2h + 1 of the thread's
-              const uint32_t x = __byte_perm(x0, x1, h ? 0x7362 : 0x5140);
-              const uint32_t y = __byte_perm(y0, y1, h ? 0x7362 : 0x5140);
-              const uint32_t af[4] = {halves<KIND, false>(x), halves<KIND, true>(x), halves<KIND, false>(y),
-                                      halves<KIND, true>(y)};
-              const int j = 2 * (w0 + v) + h;
-#pragma unroll
-              for (int n = 0; n < NT; n++) {
+            for (int n = 0; n < NT; n++) {
+              if constexpr (QT == 1) {
+                mma16816(o[j][n], af, p[g][n][0][0], p[g][n][0][1]);
+              } else {
                 float d[4];
                 mma16816_zero(d, af, p[g][n][0][0], p[g][n][0][1]);
-                if constexpr (QT == 2) mma16816(d, af, p[g][n][1][0], p[g][n][1][1]);
+                mma16816(d, af, p[g][n][1][0], p[g][n][1][1]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[j][n][e] = fmaf(d[e], vs15, o[j][n][e]);
+                for (int e = 0; e < 4; e++) o[j][n][e] += d[e];
               }
             }
           }
         }
       }
+      load_v(it + 1);
     }
-    cp_wait<0>();
+    cp_join();
     __syncwarp();
 
     // ---- the open block
     {
-      const T* kb = reinterpret_cast<const T*>(ring + st * S::STAGE);
-      const T* vb = reinterpret_cast<const T*>(ring + st * S::STAGE + S::OPENV) + r * (HDP / 8);
+      const T* kb = reinterpret_cast<const T*>(wo);
+      const T* vb = kb + 2 * hd + r * (HDP / 8);
       for (int y = 0; y < n_open; y++) {
         const int t = closed + warp + y * kQsWarps;
         if (hide && hide[t]) continue;
         const T *kr = kb + y * hd, *vr = vb + y * hd;
+        float vmax = 0.0f;  // of the token's values: the same part as a block's scale
+#pragma unroll
+        for (int d = 0; d < HDP / 8; d++)
+          if (r * (HDP / 8) + d < hd) vmax = fmaxf(vmax, fabsf(E::to(vr[d])));
+        const float lam = scale_exponent(warp_max_all(vmax));
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           float dot = 0.0f;  // of row r, over the thread's dims
@@ -775,12 +808,13 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
           for (int e = 0; e < 2; e++) {
             const float x = __shfl_sync(0xffffffffu, dot, (2 * cq + e) * 4);
             on[e] = t < seen[n][e];
-            const float mn = on[e] ? fmaxf(m[n][e], x) : m[n][e];
+            const float mn = on[e] ? fmaxf(m[n][e], x + lam) : m[n][e];
             const float ref = mn == -INFINITY ? 0.0f : mn;
             al[e] = ex2(m[n][e] - ref);
             w[e] = on[e] ? ex2(x - ref) : 0.0f;
             m[n][e] = mn;
-            l[n][e] = l[n][e] * al[e] + (r == 0 ? w[e] * 32768.0f : 0.0f);
+            l[n][e] = l[n][e] * al[e] + (r == 0 ? w[e] : 0.0f);
+            w[e] *= 16384.0f;
           }
 #pragma unroll
           for (int j = 0; j < MT; j++)
@@ -796,8 +830,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
     }
 
     // ---- merge of the warps, in order
-    __syncwarp();  // every lane is done with the ring
-    float* wo = reinterpret_cast<float*>(ring);  // [ROWS][ORow]
+    __syncwarp();  // every lane is done with the tokens in wo
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -826,8 +859,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
 #pragma unroll
       for (int w = 0; w < kQsWarps; w++) {
         const float wt = part_weight(wm[w * ROWS + row], M);
-        const float4 y = *reinterpret_cast<const float4*>(sm + (size_t)w * S::STAGES * S::STAGE +
-                                                          (row * S::ORow + d) * sizeof(float));
+        const float4 y = *reinterpret_cast<const float4*>(wo_all + w * WO + row * S::ORow + d);
         // a warp whose maximum is -inf holds zeros, or NaN from a NaN score
         L = fmaf(wt, wl[w * ROWS + row], L);
         O[0] = fmaf(wt, y.x, O[0]);
@@ -849,9 +881,9 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
       for (int x = rank * kQsWarps * 32 + tid; x < rows * (HDP / 4); x += ns * kQsWarps * 32) {
         const int row = x / (HDP / 4), d = x % (HDP / 4) * 4;
         if (d >= hd) continue;
-        float L, O[4];
+        float L, M, O[4];
         if (ns > 1) {
-          float M = -INFINITY;
+          M = -INFINITY;
 #pragma unroll 4
           for (int q = 0; q < ns; q++) M = fmaxf(M, ld_peer(peer_addr(cm_u + row * 4, q)));
           L = O[0] = O[1] = O[2] = O[3] = 0.0f;
@@ -866,18 +898,79 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 ? 1 : 2)
             O[3] = fmaf(wt, y.w, O[3]);
           }
         } else {
+          M = cm[row];
           L = cm[ROWS + row];
 #pragma unroll
           for (int e = 0; e < 4; e++) O[e] = res[row * S::ORow + d + e];
         }
-        // O is sum p v, L is 2^15 sum p; nothing seen: L = 0
-        T* y = out0 + (int64_t)(s.row0 + (x0 + row) / G) * a.out.token + (int64_t)(kvh * G + (x0 + row) % G) * a.out.head + d;
+        const int token = s.row0 + (x0 + row) / G, head = kvh * G + (x0 + row) % G;
+        if (splits > kQsCluster) {  // merged with the other clusters' by k_q8_merge
+          float* y = a.ws + (((size_t)token * a.heads + head) * groups + group) * (hd + 4);
+          *reinterpret_cast<float4*>(y + d) = make_float4(O[0], O[1], O[2], O[3]);
+          if (d == 0) {
+            y[hd] = M;
+            y[hd + 1] = L;
+          }
+          continue;
+        }
+        // O is 2^14 sum p v, L is sum p; nothing seen: L = 0
+        T* y = out0 + (int64_t)token * a.out.token + (int64_t)head * a.out.head + d;
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = E::from(L == 0.0f ? 0.0f : O[e] / (L * 3.0517578125e-05f));
+        for (int e = 0; e < 4; e++) y[e] = E::from(L == 0.0f ? 0.0f : O[e] / (L * 16384.0f));
       }
     }
     if (csize > 1) cluster_arrive_wait();  // peers are done with this CTA's result
     else __syncthreads();
+  }
+}
+
+// Merge of the clusters' results of sequences of more than kQsCluster splits,
+// in order: one warp per row and head, 4 dims a lane and step.
+template <int TYPE, int HDP>
+__global__ void __launch_bounds__(128) k_q8_merge(Q8View c, Q8Batch b, Q8Attend a, int groups) {
+  using E = Elem<TYPE>;
+  using T = typename E::T;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (w >= (int64_t)b.tokens * a.heads) return;
+  const int token = (int)(w / a.heads), head = (int)(w % a.heads);
+  int i;
+  if (b.q_start) {
+    int lo = 0, hi = b.n;  // the last i with q_start[i] <= token
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (__ldg(b.q_start + mid) <= token) lo = mid;
+      else hi = mid;
+    }
+    i = lo;
+  } else {
+    i = token / (b.tokens / b.n);
+  }
+  const Seq s = seq_of(b, c.slots, i);
+  const int len = __ldg(a.lens + i);
+  if (s.slot < 0 || token < s.row0 || token >= s.row0 + s.nrow || len < 0 || len > c.cap) return;
+  const int splits = min(qs_splits<HDP>(len & ~(kQ8Block - 1)), groups * kQsCluster);
+  if (splits <= kQsCluster) return;
+  const int n = (splits + kQsCluster - 1) / kQsCluster;
+  const float* y = a.ws + (size_t)w * groups * (c.hd + 4);
+  float M = -INFINITY;
+  for (int g = 0; g < n; g++) M = fmaxf(M, y[g * (c.hd + 4) + c.hd]);
+  for (int d = lane * 4; d < c.hd; d += 128) {
+    float L = 0.0f, O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int g = 0; g < n; g++) {
+      const float* z = y + g * (c.hd + 4);
+      const float wt = part_weight(z[c.hd], M);
+      const float4 x = *reinterpret_cast<const float4*>(z + d);
+      L = fmaf(wt, z[c.hd + 1], L);
+      O[0] = fmaf(wt, x.x, O[0]);
+      O[1] = fmaf(wt, x.y, O[1]);
+      O[2] = fmaf(wt, x.z, O[2]);
+      O[3] = fmaf(wt, x.w, O[3]);
+    }
+    T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)token * a.out.token + (int64_t)head * a.out.head + d;
+#pragma unroll
+    for (int e = 0; e < 4; e++) out[e] = E::from(L == 0.0f ? 0.0f : O[e] / (L * 16384.0f));
   }
 }
 
@@ -955,48 +1048,62 @@ bool first_on_device(unsigned long long& mask) {
   return true;
 }
 
-template <int TYPE, int KIND, int HDP, int NT>
+template <int TYPE, int KIND, int HDP, int NT, bool EXACT>
 void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st) {
-  auto kern = k_q8_attend<TYPE, KIND, HDP, NT>;
+  auto kern = k_q8_attend<TYPE, KIND, HDP, NT, EXACT>;
   constexpr size_t smem = qs_smem<HDP, NT, TYPE == kQ8F32 ? 2 : 1>();
   static unsigned long long attr = 0;
   if (first_on_device(attr)) {
     DEFER_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    DEFER_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   }
   const int64_t rows = (int64_t)std::max(b.max_q, 1) * (a.heads / c.kvh);
   const int64_t tiles = std::min<int64_t>((rows + 8 * NT - 1) / (8 * NT), 65535 / c.kvh);
-  int cl = 1;  // a power of two that holds the splits of the longest sequence
-  while (cl < qs_splits<HDP>(a.max_len / kQ8Block * kQ8Block)) cl *= 2;
-  cudaLaunchAttribute at[2];
+  const int splits = qs_splits<HDP>(a.max_len / kQ8Block * kQ8Block);  // of the longest sequence
+  const int groups = (splits + kQsCluster - 1) / kQsCluster;
+  int cl = 1;  // a power of two that holds its splits
+  while (cl < std::min(splits, kQsCluster)) cl *= 2;
+  cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = cl;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  // a cluster's CTAs on as many SMs as there are, not two on one: a single
-  // long sequence has fewer CTAs than the device has SMs
-  at[1].id = cudaLaunchAttributeClusterSchedulingPolicyPreference;
-  at[1].val.clusterSchedulingPolicyPreference = cudaClusterSchedulingPolicySpread;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(b.n * cl), (unsigned)(c.kvh * tiles), 1);
+  cfg.gridDim = dim3((unsigned)(b.n * groups * cl), (unsigned)(c.kvh * tiles), 1);
   cfg.blockDim = dim3(kQsWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
-  DEFER_CUDA(cudaLaunchKernelEx(&cfg, kern, c, b, a, (int)tiles));
+  cfg.numAttrs = 1;
+  DEFER_CUDA(cudaLaunchKernelEx(&cfg, kern, c, b, a, (int)tiles, groups));
+  if (groups > 1) k_q8_merge<TYPE, HDP><<<grid_of((int64_t)b.tokens * a.heads), 128, 0, st>>>(c, b, a, groups);
 }
 
 }  // namespace
+
+size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a) {
+  const int closed = a.max_len / kQ8Block * kQ8Block;
+  const int splits = c.hd <= 32 ? qs_splits<32>(closed) : c.hd <= 64 ? qs_splits<64>(closed)
+                     : c.hd <= 128 ? qs_splits<128>(closed) : qs_splits<256>(closed);
+  if (splits <= kQsCluster) return 0;
+  return (size_t)b.tokens * a.heads * ((splits + kQsCluster - 1) / kQsCluster) * (c.hd + 4) * sizeof(float);
+}
 
 void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st) {
   if (b.n == 0 || b.tokens == 0) return;
   const bool one = (int64_t)b.max_q * (a.heads / c.kvh) <= 8;
   dispatch(c, [&](auto type, auto kind) {
     constexpr int TY = decltype(type)::value, KI = decltype(kind)::value;
-    if (c.hd <= 32) one ? attend_few<TY, KI, 32, 1>(c, b, a, st) : attend_few<TY, KI, 32, 2>(c, b, a, st);
-    else if (c.hd <= 64) one ? attend_few<TY, KI, 64, 1>(c, b, a, st) : attend_few<TY, KI, 64, 2>(c, b, a, st);
-    else if (c.hd <= 128) one ? attend_few<TY, KI, 128, 1>(c, b, a, st) : attend_few<TY, KI, 128, 2>(c, b, a, st);
-    else attend_few<TY, KI, 256, 1>(c, b, a, st);
+    auto go = [&](auto hdp, auto exact) {
+      constexpr int HDP = decltype(hdp)::value;
+      constexpr bool EX = decltype(exact)::value != 0;
+      if (one || HDP == 256) attend_few<TY, KI, HDP, 1, EX>(c, b, a, st);
+      else attend_few<TY, KI, HDP, HDP == 256 ? 1 : 2, EX>(c, b, a, st);
+    };
+    if (c.hd == 64) go(Const<64>(), Const<1>());
+    else if (c.hd == 128) go(Const<128>(), Const<1>());
+    else if (c.hd <= 32) go(Const<32>(), Const<0>());
+    else if (c.hd <= 64) go(Const<64>(), Const<0>());
+    else if (c.hd <= 128) go(Const<128>(), Const<0>());
+    else go(Const<256>(), Const<0>());
   });
   DEFER_CUDA(cudaGetLastError());
 }

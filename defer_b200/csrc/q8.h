@@ -74,7 +74,9 @@ struct Q8Attend {
   int64_t mask_stride;
   int causal;
   float scale;
+  float* ws;  // q8_attend_workspace bytes (may be null when that is 0)
 };
+size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a);
 void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st);
 
 }  // namespace defer

@@ -163,13 +163,15 @@ def q8_read(cache: Q8Cache, k_out, v_out, lens, *, start=None, slots=None, statu
 
 
 def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: int = 0, max_len: int = 0,
-              masked=None, causal: bool = True, scale: Optional[float] = None, status=None,
+              masked=None, causal: bool = True, scale: Optional[float] = None, status=None, workspace=None,
               stream: Optional[int] = None):
     """Attention of q [tokens, heads, head_dim] over the cache into out (the
     same shape), which is returned (defer_q8_attend). lens[i] counts the
     positions of sequence i, the call's own rows among them; masked [n, cap or
     more] (uint8 or bool) hides positions; scale defaults to
-    head_dim ** -0.5."""
+    head_dim ** -0.5. Long sequences need a workspace (a contiguous device
+    array of workspace_bytes() bytes or more, used while the call runs): by
+    default it is taken from torch's allocator on the call's stream."""
     n = lens.numel()
     heads = q.shape[1] if len(q.shape) == 3 else 0
     qp, qt, qh = _rows(cache, q, heads, "q")
@@ -186,10 +188,49 @@ def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: 
         mp, ms = masked.data_ptr(), masked.stride(0) if n > 1 else 0
     b = _lib.Q8BatchC(n, tokens, max_q, _ints(cache, q_start, n + 1, "q_start"), _ints(cache, slots, n, "slots"),
                       _ints(cache, status, None, "status"))
+    if stream is None:
+        stream = _stream_of(cache.device)
+    wp, wn = None, 0
+    if workspace is not None:
+        if workspace.get_device() != cache.device or not workspace.is_contiguous():
+            _refuse("the workspace must be contiguous on the cache's device")
+        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif (max_len or cache.cap) >= _LONG:
+        wn = _workspace_bytes(cache, b, max_len, heads)
+        if wn:
+            workspace = _scratch(cache.device, wn, stream)  # freed in the stream's order
+            wp = workspace.data_ptr()
     rc = _lib.load().defer_q8_attend(cache._ref, ctypes.addressof(b), _ints(cache, lens, n, "lens"), max_len, heads,
                                      qp, qt, qh, op, ot, oh, mp, ms, 1 if causal else 0,
-                                     cache.head_dim ** -0.5 if scale is None else scale,
-                                     _stream_of(cache.device) if stream is None else stream)
+                                     cache.head_dim ** -0.5 if scale is None else scale, wp, wn, stream)
     if rc:
         _check(rc)
     return out
+
+
+_LONG = 9000  # shorter sequences need no workspace, whatever the head size
+
+
+def _workspace_bytes(cache: Q8Cache, batch, max_len: int, heads: int) -> int:
+    n = ctypes.c_size_t(0)
+    rc = _lib.load().defer_q8_attend_workspace(cache._ref, ctypes.addressof(batch), max_len, heads, ctypes.byref(n))
+    if rc:
+        _check(rc)
+    return n.value
+
+
+def workspace_bytes(cache: Q8Cache, tokens: int, heads: int, max_len: int = 0) -> int:
+    """Bytes of workspace that q8_attend of `tokens` rows of `heads` heads
+    uses with this max_len (defer_q8_attend_workspace)."""
+    z = ctypes.c_int32(0)  # rows by q_start, so that any number of them goes; it is not read
+    return _workspace_bytes(cache, _lib.Q8BatchC(1, tokens, 0, ctypes.addressof(z), None, None), max_len, heads)
+
+
+def _scratch(device: int, nbytes: int, stream: int):
+    t = sys.modules.get("torch")
+    if t is None:
+        _refuse("a sequence this long needs the workspace argument")
+    if stream == t.cuda.current_stream(device).cuda_stream:
+        return t.empty(nbytes, dtype=t.uint8, device=f"cuda:{device}")
+    with t.cuda.stream(t.cuda.ExternalStream(stream, device=device)):
+        return t.empty(nbytes, dtype=t.uint8, device=f"cuda:{device}")

@@ -337,13 +337,21 @@ DEFER_API int defer_q8_read(const defer_q8_cache* c, uint32_t n, const int32_t* 
  * at least cap): position t of sequence i is hidden where masked[i *
  * mask_stride + t] is not 0. out = sum_t p_t V_t, p = softmax(scale * q . K_t)
  * over the positions seen, 0 when there are none; softmax and sums in fp32.
- * max_len: the longest length (0: cap); it sizes the launch. A sequence's
+ * max_len: the longest length (0: cap); it sizes the launch, and a sequence
+ * that is longer is still attended as a whole. A sequence's
  * result depends on its own rows, length and cache only, not on the call's
  * other sequences. */
 DEFER_API int defer_q8_attend(const defer_q8_cache* c, const defer_q8_batch* b, const int32_t* lens,
                               uint32_t max_len, uint32_t heads, const void* q, int64_t q_token_stride,
                               int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
-                              const uint8_t* masked, int64_t mask_stride, int32_t causal, float scale, void* stream);
+                              const uint8_t* masked, int64_t mask_stride, int32_t causal, float scale,
+                              void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of 16-byte aligned device memory that such a call uses while it runs
+ * (0 unless max_len is long); its contents need no preparation and mean
+ * nothing afterwards. Calls that may run at the same time, captured graphs
+ * among them, need one each. */
+DEFER_API int defer_q8_attend_workspace(const defer_q8_cache* c, const defer_q8_batch* b, uint32_t max_len,
+                                        uint32_t heads, size_t* bytes);
 
 #ifdef __cplusplus
 }

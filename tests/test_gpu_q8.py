@@ -356,6 +356,37 @@ def test_a_sequence_does_not_depend_on_the_batch(rows):
             assert torch.equal(one, every[i * rows:(i + 1) * rows])
 
 
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F32), (256, F16)])
+def test_long_sequences_and_their_workspace(hd, dtype):
+    """More splits than a cluster holds: results through the workspace, and the same ones in any batch."""
+    longest = 20100 if hd == 64 else 11001
+    c = Case(3, 1, longest + 15 & ~15, hd, "int8", dtype, seed=hd)
+    lens = [longest, 700, longest - 1500]
+    c.append([0, 1, 2], lens)
+    for rows in (1, 2):
+        out = c.attend_check([0, 1, 2], [rows] * 3, 4)
+        q = c.randn(3 * rows, 4, hd)
+        D.q8_attend(c.cache, q, out, ints(lens))
+        for i in range(3):
+            one = torch.empty_like(q[:rows])
+            need = D.q8.workspace_bytes(c.cache, rows, 4, lens[i])
+            assert (need > 0) == (lens[i] > 9000)
+            ws = torch.full((max(need, 16),), 255, dtype=torch.uint8, device="cuda")
+            D.q8_attend(c.cache, q[i * rows:(i + 1) * rows], one, ints([lens[i]]), slots=ints([i]), max_len=lens[i],
+                        workspace=ws)
+            assert torch.equal(one, out[i * rows:(i + 1) * rows])
+        with pytest.raises(D.InvalidArgumentError, match="workspace"):
+            D.q8_attend(c.cache, q, out, ints(lens), workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    # from another stream, and a max_len that is too small: still whole sequences
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    two = torch.empty_like(out)
+    D.q8_attend(c.cache, q, two, ints(lens), stream=st.cuda_stream)
+    st.synchronize()
+    assert torch.equal(out, two)
+    c.attend_check([0, 1, 2], [1] * 3, 4, max_len=16)
+
+
 def test_strided_queries_and_outputs():
     for rows in (1, 90):
         c = Case(2, 2, 128, 64, "int8", F16)

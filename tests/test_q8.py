@@ -27,7 +27,7 @@ def batch(**kw):
 def attend(c=None, b=None, lens=P, heads=4, q=P, out=P, ot=256, oh=64, masked=None, ms=0, scale=0.125):
     c, b = c or cache(), b or batch()
     return _lib.load().defer_q8_attend(ctypes.addressof(c), ctypes.addressof(b), lens, 0, heads, q, 256, 64, out, ot,
-                                       oh, masked, ms, 1, scale, None)
+                                       oh, masked, ms, 1, scale, None, 0, None)
 
 
 def append(c=None, b=None, pos=P, k=P, v=P):
