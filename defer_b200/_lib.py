@@ -52,11 +52,6 @@ class Q8CacheC(ctypes.Structure):
                 ("v_scales", vp), ("k_tail", vp), ("v_tail", vp)]
 
 
-class Q8BatchC(ctypes.Structure):
-    _fields_ = [("n", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("max_q", ctypes.c_uint32),
-                ("q_start", vp), ("slots", vp), ("status", vp)]
-
-
 i64, u32 = ctypes.c_int64, ctypes.c_uint32
 
 TOKEN_CB = ctypes.CFUNCTYPE(ctypes.c_int, vp, ctypes.c_uint32, ctypes.c_uint64)
@@ -124,12 +119,11 @@ SIGNATURES = [
     ("defer_debug_stall", ctypes.c_int, [vp, ctypes.c_uint32]),
     ("defer_debug_tc_gemm", ctypes.c_int, [ctypes.c_int, c_f32p, ctypes.c_uint32, c_f32p, ctypes.c_uint32,
                                            ctypes.c_uint32, ctypes.c_int32, c_f32p]),
-    ("defer_q8_append", ctypes.c_int, [vp, vp, vp, vp, i64, i64, vp, i64, i64, vp]),
-    ("defer_q8_read", ctypes.c_int, [vp, u32, vp, vp, vp, vp, u32, vp, ctypes.POINTER(i64), vp, ctypes.POINTER(i64),
-                                     vp]),
-    ("defer_q8_attend", ctypes.c_int, [vp, vp, vp, u32, u32, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.c_int32,
+    ("defer_q8_append", ctypes.c_int, [vp, ctypes.c_char_p, vp, vp, i64, i64, vp, i64, i64, vp]),
+    ("defer_q8_read", ctypes.c_int, [vp, u32, vp, vp, vp, vp, u32, vp, ctypes.c_char_p, vp, ctypes.c_char_p, vp]),
+    ("defer_q8_attend", ctypes.c_int, [vp, ctypes.c_char_p, vp, u32, u32, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.c_int32,
                                        ctypes.c_float, vp, sz, vp]),
-    ("defer_q8_attend_workspace", ctypes.c_int, [vp, vp, u32, u32, c_szp]),
+    ("defer_q8_attend_workspace", ctypes.c_int, [vp, ctypes.c_char_p, u32, u32, c_szp]),
     ("defer_log_softmax_at", ctypes.c_double, [c_f32p, sz, sz]),
 ]
 

@@ -74,12 +74,14 @@ void put_bytes(const std::vector<uint8_t>& v, uint8_t* buf, size_t cap, size_t* 
 
 // The calling thread's device for the length of a call on caller's buffers.
 struct OnDevice {
-  int prev = 0;
-  explicit OnDevice(int device) {
+  int prev = 0, device;
+  explicit OnDevice(int d) : device(d) {
     DEFER_CUDA(cudaGetDevice(&prev));
     if (device != prev) DEFER_CUDA(cudaSetDevice(device));
   }
-  ~OnDevice() { cudaSetDevice(prev); }
+  ~OnDevice() {
+    if (device != prev) cudaSetDevice(prev);
+  }
   OnDevice(const OnDevice&) = delete;
   OnDevice& operator=(const OnDevice&) = delete;
 };

@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // would lose bits that a 16-bit result does not have). Softmax: running
 // maximum and sum per warp; warps, then splits, are merged in order.
 //
-// Work. The positions of the closed blocks are cut into units of 8 warp
+// Work. The positions of the closed blocks are cut into units of 4 warp
 // steps, the units into splits, one CTA each, 8 splits of a (sequence, key
 // head, row tile) forming a cluster: partial results travel through
 // distributed shared memory, and up to 8 splits need no workspace and no
@@ -306,10 +306,9 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // on to be brought into L2, which keeps enough bytes on their way. The open
 // block (fp32 or 16-bit tokens) is added at the end by the last split, a
 // token a warp, in fp32.
-constexpr int kQsWarps = 8;
+constexpr int kQsWarps = 4;
 constexpr int kQsCluster = 8;     // splits of a cluster
 constexpr int kQsMaxSplits = 64;  // of a sequence
-constexpr int kQsMinUnits = 8;    // units of a split, when there are as many
 
 template <int HDP>
 struct QsShape {
@@ -329,11 +328,14 @@ constexpr size_t qs_smem() {
          + (size_t)(8 * NT) * (3 + 2 * kQsWarps) * 4;      // row factors, m and l of the CTA and of the warps
 }
 
-// Splits of a sequence with `closed` positions in closed blocks.
+// Splits of a sequence with `closed` positions in closed blocks: of 4 units
+// or more up to 8 splits (a single short sequence is a matter of latency), of
+// 8 units or more beyond (a CTA's start and its merges cost about 5 steps).
 template <int HDP>
 __host__ __device__ __forceinline__ int qs_splits(int closed) {
-  const int n = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT / kQsMinUnits;
-  return n < 1 ? 1 : n > kQsMaxSplits ? kQsMaxSplits : n;
+  const int units = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT;
+  const int n = units < 64 ? units / 4 : units / 8;
+  return n < 1 ? 1 : units < 64 && n > kQsCluster ? kQsCluster : n > kQsMaxSplits ? kQsMaxSplits : n;
 }
 
 // Position (of 8) that row r of the score product stands for: the positions of
@@ -453,16 +455,17 @@ __device__ __forceinline__ float part_weight(float m, float M) { return m == -IN
 // EXACT: head_dim is HDP; else HDP is the next instantiated size and the
 // dims behind head_dim are zeros that are not read.
 template <int TYPE, int KIND, int HDP, int NT, bool EXACT>
-__global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 1 : 2)
+__global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
     k_q8_attend(const __grid_constant__ Q8View c, const __grid_constant__ Q8Batch b, const __grid_constant__ Q8Attend a,
                 int tiles, int groups) {
   using S = QsShape<HDP>;
   using E = Elem<TYPE>;
   using T = typename E::T;
   constexpr int QT = TYPE == kQ8F32 ? 2 : 1, ROWS = 8 * NT, MT = HDP / 16;
-  constexpr int WO = ROWS * S::ORow;  // floats of a warp's result; before that, its two tokens of the open block
+  constexpr int WO = ROWS * S::ORow;  // floats of a warp's result; before that, its tokens of the open block
   constexpr int KL = S::KW < 4 ? S::KW : 4, VL = S::VW < 4 ? S::VW : 4;  // words of one load
-  static_assert(WO * 4 >= 4 * HDP * (int)sizeof(T), "the open block's tokens fit");
+  constexpr int OPEN = kQ8Block / kQsWarps;  // tokens of the open block a warp
+  static_assert(WO * 4 >= 2 * OPEN * HDP * (int)sizeof(T), "the open block's tokens fit");
   extern __shared__ __align__(128) unsigned char sm[];
   float* wo_all = reinterpret_cast<float*>(sm);
   float* res = wo_all + kQsWarps * WO;                  // [ROWS][ORow]
@@ -513,9 +516,9 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 1 : 2)
     const int t_end = min(min(closed, most), u1 * S::UNIT);
     const int t_first = u0 * S::UNIT + warp * S::TS;
     const int steps = t_end > t_first ? (t_end - t_first + S::UNIT - 1) / S::UNIT : 0;
-    // positions of the open block that the warp adds: closed + warp (+ 8)
+    // positions of the open block that the warp adds: closed + warp, + kQsWarps, ...
     const int t_open = split == splits - 1 ? min(len, most) - closed - warp : 0;
-    const int n_open = t_open > kQsWarps ? 2 : t_open > 0 ? 1 : 0;
+    const int n_open = t_open > 0 ? (t_open + kQsWarps - 1) / kQsWarps : 0;
 
     // this thread's words of a step: K of rows r and r + 8, V of 4 positions, of each block
     uint32_t kw[S::NG][2][S::KW] = {}, vw[S::NG][4][S::VW] = {};
@@ -584,14 +587,14 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 1 : 2)
       const int row = hd * (int)sizeof(T) / 16;  // 16-byte chunks of a token
       const uint4* k16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.kt) + (sh * kQ8Block + warp) * hd);
       const uint4* v16 = reinterpret_cast<const uint4*>(static_cast<const T*>(c.vt) + (sh * kQ8Block + warp) * hd);
-      for (int x = lane; x < n_open * row; x += 32) {
-        const int y = x < row ? x : x + (kQsWarps - 1) * row;  // the second token is 8 rows on
-        cp16(smem_u32(wo) + x * 16, k16 + y);
-        cp16(smem_u32(wo) + (2 * row + x) * 16, v16 + y);
-      }
+      for (int y = 0; y < n_open; y++)
+        for (int x = lane; x < row; x += 32) {
+          cp16(smem_u32(wo) + (y * row + x) * 16, k16 + y * kQsWarps * row + x);
+          cp16(smem_u32(wo) + ((OPEN + y) * row + x) * 16, v16 + y * kQsWarps * row + x);
+        }
     }
 
-    // q rows of the tile as score operands: warp w takes rows w, w + 8
+    // q rows of the tile as score operands, a row a warp
     for (int x = warp; x < ROWS; x += kQsWarps) {
       const bool on = x0 + x < R;
       const T* q = static_cast<const T*>(a.q.p) + (int64_t)(s.row0 + (x0 + x) / G) * a.q.token +
@@ -767,7 +770,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 1 : 2)
     // ---- the open block
     {
       const T* kb = reinterpret_cast<const T*>(wo);
-      const T* vb = kb + 2 * hd + r * (HDP / 8);
+      const T* vb = kb + OPEN * hd + r * (HDP / 8);
       for (int y = 0; y < n_open; y++) {
         const int t = closed + warp + y * kQsWarps;
         if (hide && hide[t]) continue;

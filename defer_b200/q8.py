@@ -15,6 +15,7 @@ must stay allocated until the stream has run the call.
 from __future__ import annotations
 
 import ctypes
+import struct
 import sys
 from typing import Optional
 
@@ -24,7 +25,8 @@ BLOCK = 16  # positions that share a scale
 _DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
 _KINDS = {"torch.int8": 0, "torch.float8_e4m3fn": 1}
 _BYTES = ("torch.uint8", "torch.bool", "torch.int8")
-_I64x3 = ctypes.c_int64 * 3
+_BATCH = struct.Struct("=IIIxxxxQQQ")  # defer_q8_batch
+_STRIDES = struct.Struct("=qqq")
 _check = None  # the package's status check (set by defer_b200/__init__.py)
 _invalid = None
 
@@ -35,7 +37,7 @@ def _refuse(what: str):
 
 def _stream_of(device: int) -> int:
     t = sys.modules.get("torch")
-    return t.cuda.current_stream(device).cuda_stream if t is not None else 0
+    return t._C._cuda_getCurrentRawStream(device) if t is not None else 0
 
 
 _names = {}  # dtype object -> its name (str() of a torch dtype costs more than a call's other checks)
@@ -94,15 +96,21 @@ class Q8Cache:
         self._ref = ctypes.addressof(self._c)
 
 
-def _ints(cache: Q8Cache, x, n: Optional[int], what: str):
+def _ints(device: int, x, n: int, what: str) -> int:
     """Device pointer of an int32 array of n entries (None: NULL)."""
     if x is None:
-        return None
-    if _name(x) != "torch.int32" or (n is not None and x.numel() != n) or not x.is_contiguous():
-        _refuse(f"{what} must be {n} contiguous int32")
-    if x.get_device() != cache.device:
-        _refuse(f"{what} must be on the cache's device")
+        return 0
+    if _names.get(x.dtype) != "torch.int32" or x.numel() != n or x.get_device() != device or not x.is_contiguous():
+        if _name(x) != "torch.int32" or x.numel() != n or not x.is_contiguous():
+            _refuse(f"{what} must be {n} contiguous int32")
+        if x.get_device() != device:
+            _refuse(f"{what} must be on the cache's device")
     return x.data_ptr()
+
+
+def _batch(device: int, n: int, tokens: int, max_q: int, q_start, slots, status) -> bytes:
+    return _BATCH.pack(n, tokens, max_q, _ints(device, q_start, n + 1, "q_start"), _ints(device, slots, n, "slots"),
+                       0 if status is None else _ints(device, status, 1, "status"))
 
 
 def _rows(cache: Q8Cache, x, heads: int, what: str):
@@ -123,16 +131,15 @@ def q8_append(cache: Q8Cache, k, v, pos, *, q_start=None, slots=None, max_q: int
     """Writes rows k, v [tokens, kv_heads, head_dim] at positions pos[i],
     pos[i] + 1, ... of each sequence i (defer_q8_append). pos, q_start, slots
     and status are int32 device arrays."""
-    n = pos.numel()
+    dev, n = cache.device, pos.numel()
     kp, kt, kh = _rows(cache, k, cache.kv_heads, "k")
     vp, vt, vh = _rows(cache, v, cache.kv_heads, "v")
     tokens = k.shape[0]
     if v.shape[0] != tokens:
         _refuse("k and v must have the same rows")
-    b = _lib.Q8BatchC(n, tokens, max_q, _ints(cache, q_start, n + 1, "q_start"), _ints(cache, slots, n, "slots"),
-                      _ints(cache, status, None, "status"))
-    rc = _lib.load().defer_q8_append(cache._ref, ctypes.addressof(b), _ints(cache, pos, n, "pos"), kp, kt, kh, vp, vt,
-                                     vh, _stream_of(cache.device) if stream is None else stream)
+    rc = _lib.load().defer_q8_append(cache._ref, _batch(dev, n, tokens, max_q, q_start, slots, status),
+                                     _ints(dev, pos, n, "pos"), kp, kt, kh, vp, vt, vh,
+                                     _stream_of(dev) if stream is None else stream)
     if rc:
         _check(rc)
 
@@ -142,22 +149,21 @@ def q8_read(cache: Q8Cache, k_out, v_out, lens, *, start=None, slots=None, statu
     """Positions start[i] .. lens[i] - 1 of each sequence into k_out and v_out
     [n, kv_heads, rows, head_dim] (any strides of the first three); rows
     behind the last position are left as they were (defer_q8_read)."""
-    n = lens.numel()
-    shape = tuple(k_out.shape)
+    dev, n, shape = cache.device, lens.numel(), k_out.shape
     if len(shape) != 4 or shape[0] != n or shape[1] != cache.kv_heads or shape[3] != cache.head_dim:
-        _refuse(f"k_out must be [{n}, {cache.kv_heads}, rows, {cache.head_dim}], got {shape}")
-    if tuple(v_out.shape) != shape:
+        _refuse(f"k_out must be [{n}, {cache.kv_heads}, rows, {cache.head_dim}], got {tuple(shape)}")
+    if v_out.shape != shape:
         _refuse("k_out and v_out must have the same shape")
-    for x, what in ((k_out, "k_out"), (v_out, "v_out")):
-        if x.dtype != cache.dtype or x.get_device() != cache.device:
+    ks, vs = k_out.stride(), v_out.stride()
+    for x, st, what in ((k_out, ks, "k_out"), (v_out, vs, "v_out")):
+        if x.dtype != cache.dtype or x.get_device() != dev:
             _refuse(f"{what} must be {cache.dtype} on the cache's device")
-        if x.stride(3) != 1:
+        if st[3] != 1:
             _refuse(f"the head_dim elements of {what} must be contiguous")
-    rc = _lib.load().defer_q8_read(cache._ref, n, _ints(cache, lens, n, "lens"), _ints(cache, start, n, "start"),
-                                   _ints(cache, slots, n, "slots"), _ints(cache, status, None, "status"), shape[2],
-                                   k_out.data_ptr(), _I64x3(*k_out.stride()[:3]), v_out.data_ptr(),
-                                   _I64x3(*v_out.stride()[:3]),
-                                   _stream_of(cache.device) if stream is None else stream)
+    rc = _lib.load().defer_q8_read(cache._ref, n, _ints(dev, lens, n, "lens"), _ints(dev, start, n, "start"),
+                                   _ints(dev, slots, n, "slots"), 0 if status is None else _ints(dev, status, 1, "status"),
+                                   shape[2], k_out.data_ptr(), _STRIDES.pack(*ks[:3]), v_out.data_ptr(),
+                                   _STRIDES.pack(*vs[:3]), _stream_of(dev) if stream is None else stream)
     if rc:
         _check(rc)
 
@@ -172,7 +178,7 @@ def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: 
     head_dim ** -0.5. Long sequences need a workspace (a contiguous device
     array of workspace_bytes() bytes or more, used while the call runs): by
     default it is taken from torch's allocator on the call's stream."""
-    n = lens.numel()
+    dev, n = cache.device, lens.numel()
     heads = q.shape[1] if len(q.shape) == 3 else 0
     qp, qt, qh = _rows(cache, q, heads, "q")
     op, ot, oh = _rows(cache, out, heads, "out")
@@ -183,37 +189,36 @@ def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: 
     if masked is not None:
         if len(masked.shape) != 2 or masked.shape[0] != n or masked.shape[1] < cache.cap or _name(masked) not in _BYTES:
             _refuse(f"masked must be uint8 or bool [{n}, at least {cache.cap}]")
-        if masked.stride(1) != 1 or masked.get_device() != cache.device:
+        if masked.stride(1) != 1 or masked.get_device() != dev:
             _refuse("masked must be on the cache's device with contiguous rows")
         mp, ms = masked.data_ptr(), masked.stride(0) if n > 1 else 0
-    b = _lib.Q8BatchC(n, tokens, max_q, _ints(cache, q_start, n + 1, "q_start"), _ints(cache, slots, n, "slots"),
-                      _ints(cache, status, None, "status"))
+    b = _batch(dev, n, tokens, max_q, q_start, slots, status)
     if stream is None:
-        stream = _stream_of(cache.device)
+        stream = _stream_of(dev)
     wp, wn = None, 0
     if workspace is not None:
-        if workspace.get_device() != cache.device or not workspace.is_contiguous():
+        if workspace.get_device() != dev or not workspace.is_contiguous():
             _refuse("the workspace must be contiguous on the cache's device")
         wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif (max_len or cache.cap) >= _LONG:
         wn = _workspace_bytes(cache, b, max_len, heads)
         if wn:
-            workspace = _scratch(cache.device, wn, stream)  # freed in the stream's order
+            workspace = _scratch(dev, wn, stream)  # freed in the stream's order
             wp = workspace.data_ptr()
-    rc = _lib.load().defer_q8_attend(cache._ref, ctypes.addressof(b), _ints(cache, lens, n, "lens"), max_len, heads,
-                                     qp, qt, qh, op, ot, oh, mp, ms, 1 if causal else 0,
+    rc = _lib.load().defer_q8_attend(cache._ref, b, _ints(dev, lens, n, "lens"), max_len, heads, qp, qt, qh, op, ot,
+                                     oh, mp, ms, 1 if causal else 0,
                                      cache.head_dim ** -0.5 if scale is None else scale, wp, wn, stream)
     if rc:
         _check(rc)
     return out
 
 
-_LONG = 9000  # shorter sequences need no workspace, whatever the head size
+_LONG = 4500  # shorter sequences need no workspace, whatever the head size
 
 
-def _workspace_bytes(cache: Q8Cache, batch, max_len: int, heads: int) -> int:
+def _workspace_bytes(cache: Q8Cache, batch: bytes, max_len: int, heads: int) -> int:
     n = ctypes.c_size_t(0)
-    rc = _lib.load().defer_q8_attend_workspace(cache._ref, ctypes.addressof(batch), max_len, heads, ctypes.byref(n))
+    rc = _lib.load().defer_q8_attend_workspace(cache._ref, batch, max_len, heads, ctypes.byref(n))
     if rc:
         _check(rc)
     return n.value
@@ -222,8 +227,7 @@ def _workspace_bytes(cache: Q8Cache, batch, max_len: int, heads: int) -> int:
 def workspace_bytes(cache: Q8Cache, tokens: int, heads: int, max_len: int = 0) -> int:
     """Bytes of workspace that q8_attend of `tokens` rows of `heads` heads
     uses with this max_len (defer_q8_attend_workspace)."""
-    z = ctypes.c_int32(0)  # rows by q_start, so that any number of them goes; it is not read
-    return _workspace_bytes(cache, _lib.Q8BatchC(1, tokens, 0, ctypes.addressof(z), None, None), max_len, heads)
+    return _workspace_bytes(cache, _BATCH.pack(1, tokens, 0, 0, 0, 0), max_len, heads)
 
 
 def _scratch(device: int, nbytes: int, stream: int):

@@ -1,6 +1,7 @@
 """8-bit key/value cache: refusals, without a GPU. Every call here must be
 turned away by the host's checks before anything is launched."""
 import ctypes
+import struct
 
 import pytest
 
@@ -17,28 +18,25 @@ def cache(**kw):
     return c
 
 
-def batch(**kw):
-    b = _lib.Q8BatchC(2, 2, 0, None, None, None)
-    for k, v in kw.items():
-        setattr(b, k, v)
-    return b
+def batch(n=2, tokens=2):
+    return struct.pack("=IIIxxxxQQQ", n, tokens, 0, 0, 0, 0)
 
 
 def attend(c=None, b=None, lens=P, heads=4, q=P, out=P, ot=256, oh=64, masked=None, ms=0, scale=0.125):
     c, b = c or cache(), b or batch()
-    return _lib.load().defer_q8_attend(ctypes.addressof(c), ctypes.addressof(b), lens, 0, heads, q, 256, 64, out, ot,
+    return _lib.load().defer_q8_attend(ctypes.addressof(c), b, lens, 0, heads, q, 256, 64, out, ot,
                                        oh, masked, ms, 1, scale, None, 0, None)
 
 
 def append(c=None, b=None, pos=P, k=P, v=P):
     c, b = c or cache(), b or batch()
-    return _lib.load().defer_q8_append(ctypes.addressof(c), ctypes.addressof(b), pos, k, 128, 64, v, 128, 64, None)
+    return _lib.load().defer_q8_append(ctypes.addressof(c), b, pos, k, 128, 64, v, 128, 64, None)
 
 
 def read(c=None, n=2, lens=P, rows=8, ko=P, ks=(1024, 512, 64), vs=(1024, 512, 64)):
-    a = ctypes.c_int64 * 3
     c = c or cache()
-    return _lib.load().defer_q8_read(ctypes.addressof(c), n, lens, None, None, None, rows, ko, a(*ks), P, a(*vs), None)
+    return _lib.load().defer_q8_read(ctypes.addressof(c), n, lens, None, None, None, rows, ko, struct.pack("=qqq", *ks), P,
+                                      struct.pack("=qqq", *vs), None)
 
 
 BAD = D.InvalidArgumentError.code
@@ -56,7 +54,7 @@ def test_a_bad_cache_is_refused(field, value):
 def test_null_descriptors_are_refused():
     L = _lib.load()
     b = batch()
-    assert L.defer_q8_append(None, ctypes.addressof(b), P, P, 128, 64, P, 128, 64, None) == BAD
+    assert L.defer_q8_append(None, b, P, P, 128, 64, P, 128, 64, None) == BAD
     c = cache()
     assert L.defer_q8_append(ctypes.addressof(c), None, P, P, 128, 64, P, 128, 64, None) == BAD
 
