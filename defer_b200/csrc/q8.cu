@@ -10,11 +10,6 @@
 // The product with r instead of a division keeps the writer at one
 // multiplication an element; it moves a value across a rounding border only
 // within 2^-23 of it.
-#include "q8.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -22,33 +17,12 @@
 #include <cmath>
 
 #include "common.h"
+#include "q8.cuh"
 
 namespace defer {
 namespace {
 
 constexpr float kQ8Tiny = 6.018531076210112e-36f;  // 2^-117
-
-// ------------------------------------------------------------- elements
-template <int TYPE>
-struct Elem;
-template <>
-struct Elem<kQ8F32> {
-  using T = float;
-  static __device__ __forceinline__ float to(float x) { return x; }
-  static __device__ __forceinline__ float from(float x) { return x; }
-};
-template <>
-struct Elem<kQ8Bf16> {
-  using T = __nv_bfloat16;
-  static __device__ __forceinline__ float to(T x) { return __bfloat162float(x); }
-  static __device__ __forceinline__ T from(float x) { return __float2bfloat16_rn(x); }
-};
-template <>
-struct Elem<kQ8F16> {
-  using T = __half;
-  static __device__ __forceinline__ float to(T x) { return __half2float(x); }
-  static __device__ __forceinline__ T from(float x) { return __float2half_rn(x); }
-};
 
 // Code byte of t = x * r, and the value of a code byte.
 template <int KIND>
@@ -67,40 +41,6 @@ __device__ __forceinline__ float decode(uint32_t byte) {
   } else {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
   }
-}
-
-__device__ __forceinline__ float warp_max_all(float v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
-}
-
-// Sequence i of a call: its slot and its rows. kSeqSkip: padding or rows out
-// of range, nothing is touched; kSeqBad: valid rows of a bad slot.
-constexpr int kSeqSkip = -1, kSeqBad = -2;
-struct Seq {
-  int slot, row0, nrow;
-};
-__device__ __forceinline__ Seq seq_of(const Q8Batch& b, int slots, int i) {
-  Seq s;
-  s.slot = b.slots ? max(__ldg(b.slots + i), kSeqSkip) : i;
-  if (s.slot >= slots) {
-    if (b.status) atomicOr(b.status, (int)kQ8BadRange);
-    s.slot = kSeqBad;
-  }
-  if (b.q_start) {
-    s.row0 = __ldg(b.q_start + i);
-    const int end = __ldg(b.q_start + i + 1);
-    s.nrow = end - s.row0;
-    if (s.row0 < 0 || end < s.row0 || end > b.tokens) {
-      if (b.status) atomicOr(b.status, (int)kQ8BadRange);
-      s.slot = kSeqSkip;
-    }
-  } else {
-    s.nrow = b.tokens / b.n;
-    s.row0 = i * s.nrow;
-  }
-  return s;
 }
 
 // ------------------------------------------------------------------ append
@@ -343,7 +283,6 @@ __host__ __device__ __forceinline__ int qs_splits(int closed) {
 // neighbours.
 __device__ __forceinline__ int qs_row(int r) { return (r >> 1) + (r & 1) * 4; }
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -384,32 +323,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 of 16 bit
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two fp16 numbers from code bytes (SEL: the prmt selector that puts two
-// bytes x, y as x . y . into 16-bit lanes). int8: the byte with its sign bit
-// flipped is x + 128; 0x6400 | u is 1024 + u, so one subtraction of 1152
-// leaves x, exactly. `w` comes from flip<KIND>.
-template <int KIND>
-__device__ __forceinline__ uint32_t flip(uint32_t w) {
-  return KIND == kQ8Int8 ? w ^ 0x80808080u : w;
-}
-template <int KIND, bool HI>
-__device__ __forceinline__ uint32_t halves(uint32_t w) {
-  if constexpr (KIND == kQ8Int8) {
-    const uint32_t u = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
-    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480))));
-  } else {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? w >> 16 : w & 0xFFFFu), __NV_E4M3);
-    return h2_bits(__half2(h));
-  }
-}
-
 __device__ __forceinline__ void cluster_arrive_wait() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -442,11 +355,6 @@ __device__ __forceinline__ float4 ld_peer4(uint32_t a) {
                : "r"(a)
                : "memory");
   return v;
-}
-
-// Exponent of a value scale (floor of its base-2 logarithm), from -100 up.
-__device__ __forceinline__ float scale_exponent(float v) {
-  return (float)max((__float_as_int(v) >> 23) - 127, -100);
 }
 
 // Weight of a partial result with maximum m under the total's maximum M.
@@ -484,6 +392,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
   const int G = a.heads / c.kvh, R = s.nrow * G;
   if (s.slot == kSeqSkip || R == 0) return;
   if (s.slot == kSeqBad) len = -1;
+  if (a.tiled && R > kQ8FewRows) return;
   T* const out0 = static_cast<T*>(const_cast<void*>(a.out.p));
   if (len < 0 || len > c.cap) {
     if (b.status && tid == 0) atomicOr(b.status, (int)kQ8BadRange);
@@ -952,6 +861,7 @@ __global__ void __launch_bounds__(128) k_q8_merge(Q8View c, Q8Batch b, Q8Attend 
   const Seq s = seq_of(b, c.slots, i);
   const int len = __ldg(a.lens + i);
   if (s.slot < 0 || token < s.row0 || token >= s.row0 + s.nrow || len < 0 || len > c.cap) return;
+  if (a.tiled && s.nrow * (a.heads / c.kvh) > kQ8FewRows) return;
   const int splits = min(qs_splits<HDP>(len & ~(kQ8Block - 1)), groups * kQsCluster);
   if (splits <= kQsCluster) return;
   const int n = (splits + kQsCluster - 1) / kQsCluster;
@@ -1083,6 +993,7 @@ void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream
 }  // namespace
 
 size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a) {
+  if (!b.q_start && q8_tiles(c, b, a)) return 0;
   const int closed = a.max_len / kQ8Block * kQ8Block;
   const int splits = c.hd <= 32 ? qs_splits<32>(closed) : c.hd <= 64 ? qs_splits<64>(closed)
                      : c.hd <= 128 ? qs_splits<128>(closed) : qs_splits<256>(closed);
@@ -1090,8 +1001,16 @@ size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a)
   return (size_t)b.tokens * a.heads * ((splits + kQsCluster - 1) / kQsCluster) * (c.hd + 4) * sizeof(float);
 }
 
-void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st) {
+void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& args, cudaStream_t st) {
   if (b.n == 0 || b.tokens == 0) return;
+  Q8Attend a = args;
+  a.out_aligned = aligned16(a.out.p, a.out.token, a.out.head, 0, esize_of(c.type));
+  a.q_aligned = aligned16(a.q.p, a.q.token, a.q.head, 0, esize_of(c.type));
+  a.tiled = q8_tiles(c, b, a);
+  if (a.tiled) {
+    q8_attend_tiles(c, b, a, st);
+    if (!b.q_start) return;  // every sequence has the same number of rows: none is left
+  }
   const bool one = (int64_t)b.max_q * (a.heads / c.kvh) <= 8;
   dispatch(c, [&](auto type, auto kind) {
     constexpr int TY = decltype(type)::value, KI = decltype(kind)::value;

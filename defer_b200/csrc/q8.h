@@ -25,6 +25,7 @@ enum Q8Type : int { kQ8F32 = 0, kQ8Bf16 = 1, kQ8F16 = 2 };
 enum Q8Status : int {
   kQ8BadRange = 1,   // slot, length, position or row range outside its bounds
   kQ8SlotTwice = 2,  // append: the slot appears in an earlier sequence of the call
+  kQ8Timeout = 4,    // attend: a bounded wait ran out; the rows are NaN
 };
 
 // One layer's buffers (every pointer 16-byte aligned device memory).
@@ -75,7 +76,17 @@ struct Q8Attend {
   int causal;
   float scale;
   float* ws;  // q8_attend_workspace bytes (may be null when that is 0)
+  // set by q8_attend
+  int q_aligned, out_aligned;  // the rows start on 16 bytes
+  int tiled;                   // sequences of more than kQ8FewRows rows are q8_attend_tiles'
 };
+// Rows of a sequence and key head up to which the streaming kernel takes them
+// all: 4 passes over the cache with 16 rows each.
+constexpr int kQ8FewRows = 64;
+// Whether a call may hold sequences for the tile kernel (q8_tile.cu), and that
+// kernel's launch for them.
+bool q8_tiles(const Q8View& c, const Q8Batch& b, const Q8Attend& a);
+void q8_attend_tiles(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st);
 size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a);
 void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st);
 
