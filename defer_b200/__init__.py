@@ -11,7 +11,8 @@ C ABI in include/defer_b200.h:
     seed_from_u64, words_per_sample, sample_logits      (src/engine.rs, src/sampler.rs)
     DeferCheckpoint, WalHeader, WalWriter, WalLog       (src/checkpoint.rs, src/wal.rs)
     ablation_attribution, log_softmax_at                (src/attribution.rs)
-    Q8Cache, q8_append, q8_read, q8_attend              (no counterpart: a key/value cache in 8 bits)
+    QuantKvCache, Model.new_quant_cache / forward_q8,
+    Q8Cache, q8_append, q8_read, q8_attend              (no counterpart: key/value caches in 8 bits)
 
 plus the batched drivers (replay_batch, generate_batch) that advance many
 sessions per device step. Every call runs the CUDA path; there is no CPU
@@ -36,7 +37,7 @@ __all__ = [
     "Config", "Model", "KvCache", "Session", "DeferCheckpoint", "WalHeader", "WalWriter", "WalLog",
     "seed_from_u64", "chacha8_words", "words_per_sample", "sample_logits", "log_softmax_at",
     "ablation_attribution", "replay_batch", "generate_batch",
-    "Q8Cache", "q8_append", "q8_read", "q8_attend",
+    "QuantKvCache", "Q8Cache", "q8_append", "q8_read", "q8_attend",
 ]
 
 
@@ -198,6 +199,28 @@ class Model:
     def forward(self, token: int, cache: "KvCache"):
         return self.forward_ext(token, cache, ())
 
+    def new_quant_cache(self, slots: int = 1, cap: int = 0, kind: str = "int8") -> "QuantKvCache":
+        """Caches of `slots` sessions in 8 bits ("int8" or "e4m3" codes)."""
+        if kind not in ("int8", "e4m3"):
+            raise InvalidArgumentError(f"kind must be 'int8' or 'e4m3', got {kind!r}")
+        h = ctypes.c_void_p()
+        _check(_L().defer_qcache_new(self._h, slots, cap, 0 if kind == "int8" else 1, ctypes.byref(h)))
+        return QuantKvCache(h, self, slots, kind)
+
+    def forward_q8(self, tokens: Sequence[int], cache: "QuantKvCache", slots: Optional[Sequence[int]] = None,
+                   logits: bool = True):
+        """One token in each of `slots` (0, 1, ... by default) with attention
+        over the 8-bit cache; returns logits [len(tokens), vocab]."""
+        n = len(tokens)
+        slots = range(n) if slots is None else slots
+        if len(slots) != n:
+            raise InvalidArgumentError("one token for each slot")
+        out = np.empty((n, self.config.vocab_size), np.float32) if logits else None
+        ka, kp = _u32arr(slots)
+        ta, tp = _u32arr(tokens)
+        _check(_L().defer_forward_q8(self._h, cache._h, kp, tp, n, _f32p(out) if logits else None))
+        return out
+
     def timing(self, reset: bool = False) -> dict:
         """Totals of the token-loop runs since the last reset: device_ms
         (CUDA events on the model's stream), runs, launches, tokens and
@@ -285,6 +308,53 @@ class KvCache:
         e = ctypes.c_int(0)
         _check(_L().defer_cache_bit_eq(self._h, other._h, ctypes.byref(e)))
         return bool(e.value)
+
+
+class QuantKvCache:
+    """Key/value caches of several sessions of a model in 8 bits, in HBM:
+    blocks of 16 positions share one scale per layer and head; the block that
+    is still open is held in fp32."""
+
+    def __init__(self, handle, model: Model, slots: int, kind: str):
+        self._h = handle
+        self.model = model
+        self.slots = slots
+        self.kind = kind
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            _L().defer_qcache_free(h)
+        self._h = None
+
+    def len(self, slot: int = 0) -> int:
+        return _L().defer_qcache_len(self._h, slot)
+
+    def truncate(self, n: int, slot: int = 0):
+        _check(_L().defer_qcache_truncate(self._h, slot, n))
+
+    def store(self, cache: KvCache, slot: int = 0):
+        """Quantises a KvCache of the same model into the slot."""
+        _check(_L().defer_qcache_store(self._h, slot, cache._h))
+
+    def load(self, slot: int = 0) -> KvCache:
+        """The slot's values as a new KvCache."""
+        h = ctypes.c_void_p()
+        _check(_L().defer_qcache_load(self._h, slot, ctypes.byref(h)))
+        return KvCache(h, self.model, owned=True)
+
+    def layer(self, l: int, slot: int = 0):
+        n = self.len(slot) * self.model.config.kv_dim
+        k = np.empty(max(n, 1), np.float32)
+        v = np.empty(max(n, 1), np.float32)
+        _check(_L().defer_qcache_download(self._h, slot, l, _f32p(k), _f32p(v)))
+        return k[:n], v[:n]
+
+    def view(self, l: int) -> "_lib.Q8CacheC":
+        """One layer's device buffers (defer_q8_cache)."""
+        out = _lib.Q8CacheC()
+        _check(_L().defer_qcache_view(self._h, l, ctypes.byref(out)))
+        return out
 
 
 # ----------------------------------------------------------- sampler / PRNG

@@ -124,6 +124,15 @@ SIGNATURES = [
     ("defer_q8_attend", ctypes.c_int, [vp, ctypes.c_char_p, vp, u32, u32, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.c_int32,
                                        ctypes.c_float, vp, sz, vp]),
     ("defer_q8_attend_workspace", ctypes.c_int, [vp, ctypes.c_char_p, u32, u32, c_szp]),
+    ("defer_qcache_new", ctypes.c_int, [vp, u32, u32, ctypes.c_int32, ctypes.POINTER(vp)]),
+    ("defer_qcache_free", None, [vp]),
+    ("defer_qcache_len", sz, [vp, u32]),
+    ("defer_qcache_truncate", ctypes.c_int, [vp, u32, sz]),
+    ("defer_qcache_store", ctypes.c_int, [vp, u32, vp]),
+    ("defer_qcache_load", ctypes.c_int, [vp, u32, ctypes.POINTER(vp)]),
+    ("defer_qcache_download", ctypes.c_int, [vp, u32, u32, c_f32p, c_f32p]),
+    ("defer_qcache_view", ctypes.c_int, [vp, u32, ctypes.POINTER(Q8CacheC)]),
+    ("defer_forward_q8", ctypes.c_int, [vp, vp, c_u32p, c_u32p, sz, c_f32p]),
     ("defer_log_softmax_at", ctypes.c_double, [c_f32p, sz, sz]),
 ]
 

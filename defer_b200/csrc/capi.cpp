@@ -33,6 +33,9 @@ struct defer_session {
   std::unique_ptr<defer::Session> s;
   defer_cache cache_view;
 };
+struct defer_qcache {
+  std::unique_ptr<defer::QuantCache> c;
+};
 struct defer_wal_writer {
   std::unique_ptr<defer::WalWriter> w;
 };
@@ -777,6 +780,85 @@ int defer_q8_attend(const defer_q8_cache* cache, const defer_q8_batch* batch, co
              "the workspace is smaller than defer_q8_attend_workspace, or not 16-byte aligned");
     OnDevice on(cache->device);
     defer::q8_attend(c, b, a, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int defer_qcache_new(defer_model* m, uint32_t slots, uint32_t cap, int32_t kind, defer_qcache** out) {
+  return guard([&] {
+    need(m, "model");
+    need(out, "out");
+    q8_check(cap <= 1u << 30 && slots <= 1u << 24, "cap must be at most 2^30, slots at most 2^24");
+    std::unique_ptr<defer_qcache> h(new defer_qcache());
+    h->c.reset(defer::qcache_new(m->m.get(), (int)slots, (int)cap, kind));
+    *out = h.release();
+  });
+}
+
+void defer_qcache_free(defer_qcache* c) { delete c; }
+
+size_t defer_qcache_len(const defer_qcache* c, uint32_t slot) {
+  return c && slot < c->c->len.size() ? c->c->len[slot] : 0;
+}
+
+int defer_qcache_truncate(defer_qcache* c, uint32_t slot, size_t n) {
+  return guard([&] {
+    need(c, "cache");
+    defer::qcache_truncate(c->c.get(), slot, n);
+  });
+}
+
+int defer_qcache_store(defer_qcache* c, uint32_t slot, const defer_cache* src) {
+  return guard([&] {
+    need(c, "cache");
+    need(src, "src");
+    defer::qcache_store(c->c.get(), slot, src->c);
+  });
+}
+
+int defer_qcache_load(const defer_qcache* c, uint32_t slot, defer_cache** out) {
+  return guard([&] {
+    need(c, "cache");
+    need(out, "out");
+    std::unique_ptr<defer_cache> h(new defer_cache());
+    h->c = defer::qcache_load(c->c.get(), slot);
+    *out = h.release();
+  });
+}
+
+int defer_qcache_download(const defer_qcache* c, uint32_t slot, uint32_t layer, float* keys, float* values) {
+  return guard([&] {
+    need(c, "cache");
+    if (layer >= c->c->model->cfg.num_layers) defer::fail(defer::kInvalidArgument, "layer out of range");
+    if (defer_qcache_len(c, slot)) {
+      need(keys, "keys");
+      need(values, "values");
+    }
+    defer::qcache_download(c->c.get(), slot, (int)layer, keys, values);
+  });
+}
+
+int defer_qcache_view(const defer_qcache* c, uint32_t layer, defer_q8_cache* out) {
+  return guard([&] {
+    need(c, "cache");
+    need(out, "out");
+    if (layer >= c->c->model->cfg.num_layers) defer::fail(defer::kInvalidArgument, "layer out of range");
+    const defer::Q8View v = c->c->view((int)layer);
+    *out = {c->c->model->device, v.kind, v.type, (uint32_t)v.slots, (uint32_t)v.kvh, (uint32_t)v.cap, (uint32_t)v.hd,
+            v.kc, v.vc, v.ks, v.vs, v.kt, v.vt};
+  });
+}
+
+int defer_forward_q8(defer_model* m, defer_qcache* c, const uint32_t* slots, const uint32_t* tokens, size_t n,
+                     float* logits_out) {
+  return guard([&] {
+    need(m, "model");
+    need(c, "cache");
+    if (c->c->model != m->m.get()) defer::fail(defer::kInvalidArgument, "cache belongs to another model");
+    if (n) {
+      need(slots, "slots");
+      need(tokens, "tokens");
+    }
+    defer::forward_q8(c->c.get(), slots, tokens, n, logits_out);
   });
 }
 

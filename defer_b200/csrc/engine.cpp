@@ -87,6 +87,7 @@ Runner::~Runner() {
   cudaFree(logits_);
   cudaFree(part_);
   cudaFree(d_sess_);
+  if (d_staged_) cudaFree(d_staged_);
   cudaFree(d_state_);
   cudaFree(d_ctrl_);
   if (flow_words_) cudaFree(flow_words_);
@@ -629,6 +630,312 @@ void model_forward(Model* m, KvCache* c, uint32_t token, const size_t* masked, s
   fr->run(progs, res);
   if (any) DEFER_CUDA(cudaMemset(c->mask, 0, bits.size() * 4));
   if (logits_out) fr->download_logits(0, logits_out);
+}
+
+// ------------------------------------------------------- cache in 8 bits
+namespace {
+// Bytes of one layer's arrays of one of K and V, each rounded up to 256.
+struct QSizes {
+  size_t codes, scales, tail, layer;
+  QSizes(const Model* m, int slots, int cap) {
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    const size_t rows = (size_t)slots * m->cfg.num_kv_heads;
+    codes = up(rows * cap * m->cfg.head_dim);
+    scales = up(rows * (cap / kQ8Block) * sizeof(float));
+    tail = up(rows * kQ8Block * m->cfg.head_dim * sizeof(float));
+    layer = 2 * (codes + scales + tail);
+  }
+};
+
+// The ints of a call on one slot: {pos or start, length, slot}.
+void one_slot(const QuantCache* c, int a, int len, int slot) {
+  const int v[3] = {a, len, slot};
+  DEFER_CUDA(cudaMemcpyAsync(c->ints, v, sizeof(v), cudaMemcpyHostToDevice, c->model->stream));
+}
+
+void need_slot(const QuantCache* c, uint32_t slot) {
+  if (slot >= (uint32_t)c->slots) fail(kInvalidArgument, "slot " + std::to_string(slot) + " out of range");
+}
+}  // namespace
+
+QuantCache::~QuantCache() {
+  if (mem) cudaFree(mem);
+  if (ints) cudaFree(ints);
+  if (stage) cudaFree(stage);
+  if (ws) cudaFree(ws);
+}
+
+Q8View QuantCache::view(int layer) const {
+  const QSizes z(model, slots, cap);
+  unsigned char* p = mem + (size_t)layer * z.layer;
+  Q8View v;
+  v.kc = p;
+  v.vc = p + z.codes;
+  p += 2 * z.codes;
+  v.ks = reinterpret_cast<float*>(p);
+  v.vs = reinterpret_cast<float*>(p + z.scales);
+  p += 2 * z.scales;
+  v.kt = p;
+  v.vt = p + z.tail;
+  v.slots = slots;
+  v.kvh = (int)model->cfg.num_kv_heads;
+  v.cap = cap;
+  v.hd = (int)model->cfg.head_dim;
+  v.kind = kind;
+  v.type = kQ8F32;
+  return v;
+}
+
+QuantCache* qcache_new(const Model* m, int slots, int cap, int kind) {
+  if (slots < 1 || slots > 1 << 24) fail(kInvalidArgument, "slots must be 1 to 2^24");
+  if (kind != kQ8Int8 && kind != kQ8E4m3) fail(kInvalidArgument, "kind must be 0 (int8) or 1 (e4m3)");
+  const uint32_t hd = m->cfg.head_dim;
+  if (hd % 16 || hd > (uint32_t)kQ8MaxHeadDim)
+    fail(kInvalidArgument, "8-bit caches need a head_dim that is a multiple of 16 up to 256; this model has " +
+                               std::to_string(hd));
+  if (cap <= 0) cap = (int)m->cfg.max_seq_len;
+  if (cap > 1 << 30) fail(kInvalidArgument, "cache capacity too large");
+  cap = (cap + kQ8Block - 1) / kQ8Block * kQ8Block;
+  DEFER_CUDA(cudaSetDevice(m->device));
+  std::unique_ptr<QuantCache> c(new QuantCache());
+  c->model = m;
+  c->slots = slots;
+  c->cap = cap;
+  c->kind = kind;
+  c->len.assign(slots, 0);
+  DEFER_CUDA(cudaMalloc(&c->mem, QSizes(m, slots, cap).layer * m->cfg.num_layers));
+  DEFER_CUDA(cudaMalloc(&c->ints, (size_t)3 * std::max(slots, 1) * sizeof(int)));
+  return c.release();
+}
+
+void qcache_truncate(QuantCache* c, uint32_t slot, size_t n) {
+  need_slot(c, slot);
+  const size_t len = c->len[slot];
+  if (n >= len) return;
+  const int rows = (int)(n % kQ8Block), start = (int)n - rows;
+  if (rows && n / kQ8Block < len / kQ8Block) {
+    // the block of position n was closed: its first `rows` positions become the tail
+    DEFER_CUDA(cudaSetDevice(c->model->device));
+    one_slot(c, start, (int)len, (int)slot);
+    for (uint32_t l = 0; l < c->model->cfg.num_layers; l++) {
+      const Q8View v = c->view((int)l);
+      const int64_t head = (int64_t)kQ8Block * v.hd;
+      const size_t at = (size_t)slot * v.kvh * head;
+      q8_read(v, 1, c->ints + 1, c->ints, c->ints + 2, nullptr, rows, {static_cast<float*>(v.kt) + at, 0, v.hd, head},
+              {static_cast<float*>(v.vt) + at, 0, v.hd, head}, c->model->stream);
+    }
+    DEFER_CUDA(cudaStreamSynchronize(c->model->stream));
+  }
+  c->len[slot] = n;
+}
+
+void qcache_store(QuantCache* c, uint32_t slot, const KvCache* src) {
+  need_slot(c, slot);
+  if (src->model != c->model) fail(kInvalidArgument, "caches of different models");
+  if (src->len > (size_t)c->cap) fail(kModel, "cache capacity " + std::to_string(c->cap) + " exceeded");
+  const Model* m = c->model;
+  DEFER_CUDA(cudaSetDevice(m->device));
+  c->len[slot] = 0;
+  if (src->len) {
+    one_slot(c, 0, (int)src->len, (int)slot);
+    for (uint32_t l = 0; l < m->cfg.num_layers; l++) {
+      const Q8View v = c->view((int)l);
+      const int64_t head = (int64_t)src->cap * v.hd;
+      const Q8Batch b{1, (int)src->len, (int)src->len, nullptr, c->ints + 2, nullptr};
+      q8_append(v, b, c->ints, {src->k + l * src->layer_stride(), v.hd, head},
+                {src->v + l * src->layer_stride(), v.hd, head}, m->stream);
+    }
+    DEFER_CUDA(cudaStreamSynchronize(m->stream));
+  }
+  c->len[slot] = src->len;
+}
+
+KvCache* qcache_load(const QuantCache* c, uint32_t slot) {
+  need_slot(c, slot);
+  const Model* m = c->model;
+  std::unique_ptr<KvCache> dst(cache_new(m, c->cap));
+  const size_t len = c->len[slot];
+  if (len) {
+    one_slot(c, 0, (int)len, (int)slot);
+    for (uint32_t l = 0; l < m->cfg.num_layers; l++) {
+      const Q8View v = c->view((int)l);
+      const int64_t head = (int64_t)dst->cap * v.hd;
+      q8_read(v, 1, c->ints + 1, nullptr, c->ints + 2, nullptr, (int)len,
+              {dst->k + l * dst->layer_stride(), 0, v.hd, head}, {dst->v + l * dst->layer_stride(), 0, v.hd, head},
+              m->stream);
+    }
+    DEFER_CUDA(cudaStreamSynchronize(m->stream));
+  }
+  dst->len = len;
+  return dst.release();
+}
+
+void qcache_download(const QuantCache* c, uint32_t slot, int layer, float* keys, float* values) {
+  need_slot(c, slot);
+  const Model* m = c->model;
+  const size_t len = c->len[slot], n = len * m->cfg.kv_dim();
+  if (!len) return;
+  DEFER_CUDA(cudaSetDevice(m->device));
+  struct Buf {
+    float* p = nullptr;
+    ~Buf() {
+      if (p) cudaFree(p);
+    }
+  } buf;
+  DEFER_CUDA(cudaMalloc(&buf.p, 2 * n * sizeof(float)));
+  one_slot(c, 0, (int)len, (int)slot);
+  const Q8View v = c->view(layer);
+  const int64_t row = m->cfg.kv_dim();
+  q8_read(v, 1, c->ints + 1, nullptr, c->ints + 2, nullptr, (int)len, {buf.p, 0, row, v.hd}, {buf.p + n, 0, row, v.hd},
+          m->stream);
+  DEFER_CUDA(cudaMemcpyAsync(keys, buf.p, n * sizeof(float), cudaMemcpyDeviceToHost, m->stream));
+  DEFER_CUDA(cudaMemcpyAsync(values, buf.p + n, n * sizeof(float), cudaMemcpyDeviceToHost, m->stream));
+  DEFER_CUDA(cudaStreamSynchronize(m->stream));
+}
+
+void Runner::step_q8(QuantCache& qc, const uint32_t* slots, const uint32_t* tokens, int n) {
+  if (n > B_) fail(kInvalidArgument, "more slots than the runner has");
+  if (m_->tc_all && n > kTcM) fail(kInvalidArgument, "runs of this model take at most 128 slots (tensor-core step)");
+  DEFER_CUDA(cudaSetDevice(m_->device));
+  cudaStream_t st = m_->stream;
+  const DModel& d = m_->dm;
+  if (!d_staged_) DEFER_CUDA(cudaMalloc(&d_staged_, sizeof(DSession) * B_));
+  if ((size_t)n > scratch_words_ || !d_scratch_) {
+    if (d_scratch_) cudaFree(d_scratch_);
+    d_scratch_ = nullptr;
+    scratch_words_ = std::max<size_t>(n, 4096);
+    DEFER_CUDA(cudaMalloc(&d_scratch_, scratch_words_ * 4));
+  }
+  const size_t row = (size_t)d.L * d.KVD;
+  if (!qc.stage) DEFER_CUDA(cudaMalloc(&qc.stage, 2 * (size_t)qc.slots * row * sizeof(float)));
+  std::vector<DSession> sess(n), staged(n);
+  std::vector<DSlotState> state(n);
+  std::vector<int> ints((size_t)3 * n);
+  int most = 0;
+  double kv_read = 0.0;
+  for (int b = 0; b < n; b++) {
+    const int pos = (int)qc.len[slots[b]];
+    DSession& s = sess[b];
+    memset(&s, 0, sizeof(s));
+    s.tokens = d_scratch_ + b;
+    s.cap = qc.cap;
+    s.pos = pos;
+    s.n_prompt = s.n_total = 1;
+    s.lanes = 1;
+    // The QKV epilogue stores the K (V) row of layer l, head h at
+    // kc + ((l * heads + h) * cap + pos) * head_dim: with a capacity of one
+    // position, and kc `pos` rows in front of it, that is the slot's place
+    // [layer][head] in the stage.
+    DSession& z = staged[b];
+    z = s;
+    z.cap = 1;
+    const size_t back = (size_t)pos * d.HD * sizeof(float);
+    z.kc = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(qc.stage + (size_t)b * row) - back);
+    z.vc = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(qc.stage + ((size_t)qc.slots + b) * row) - back);
+    memset(&state[b], 0, sizeof(state[b]));
+    state[b].pos = pos;
+    state[b].div_step = -1;
+    ints[b] = pos;
+    ints[n + b] = pos + 1;
+    ints[2 * n + b] = (int)slots[b];
+    most = std::max(most, pos + 1);
+    kv_read += (double)(pos + 1) * d.L * 2.0 * d.NKV * (d.HD + 4.0 / kQ8Block);
+  }
+  const Q8Batch batch{n, n, 1, nullptr, qc.ints + 2 * n, nullptr};
+  Q8Attend a{};
+  a.lens = qc.ints + n;
+  a.max_len = most;
+  a.heads = d.NH;
+  a.q = {q_, d.QD, d.HD};
+  a.out = {att_, d.QD, d.HD};
+  a.causal = 1;
+  a.scale = d.scale;
+  const size_t need = q8_attend_workspace(qc.view(0), batch, a);
+  if (need > qc.ws_bytes) {
+    if (qc.ws) cudaFree(qc.ws);
+    qc.ws = nullptr;
+    qc.ws_bytes = 0;
+    DEFER_CUDA(cudaMalloc(&qc.ws, need));
+    qc.ws_bytes = need;
+  }
+  a.ws = qc.ws;
+  DEFER_CUDA(cudaMemcpyAsync(d_scratch_, tokens, (size_t)n * 4, cudaMemcpyHostToDevice, st));
+  DEFER_CUDA(cudaMemcpyAsync(d_sess_, sess.data(), sizeof(DSession) * n, cudaMemcpyHostToDevice, st));
+  DEFER_CUDA(cudaMemcpyAsync(d_staged_, staged.data(), sizeof(DSession) * n, cudaMemcpyHostToDevice, st));
+  DEFER_CUDA(cudaMemcpyAsync(d_state_, state.data(), sizeof(DSlotState) * n, cudaMemcpyHostToDevice, st));
+  DEFER_CUDA(cudaMemcpyAsync(qc.ints, ints.data(), ints.size() * sizeof(int), cudaMemcpyHostToDevice, st));
+  DEFER_CUDA(cudaMemsetAsync(d_ctrl_, 0, 8 * sizeof(int), st));
+  DBatch bt{};
+  bt.B = n;
+  bt.sess = d_sess_;
+  bt.st = d_state_;
+  bt.x = x_;
+  bt.tickets = tickets_;
+  bt.nblk = nblk_;
+  const size_t per = (size_t)n * nblk_;
+  bt.ss.lmax = stats_;
+  bt.ss.larg = reinterpret_cast<int*>(stats_ + per);
+  bt.ss.smax = stats_ + 2 * per;
+  bt.ss.esum = stats_ + 3 * per;
+  bt.ss.psum = stats_ + 4 * per;
+  bt.q = q_;
+  bt.att = att_;
+  bt.g = g_;
+  bt.logits = logits_;
+  bt.part = part_;
+  bt.max_chunks = max_chunks_;
+  bt.status = d_ctrl_;
+  bt.any_active = d_ctrl_ + 1;
+  bt.bar = reinterpret_cast<unsigned*>(d_ctrl_ + 3);
+  bt.parts = 1;
+  bt.trace_step = -1;
+  DBatch bs = bt;
+  bs.sess = d_staged_;
+  auto attn = [&](int l) {
+    const Q8View v = qc.view(l);
+    q8_append(v, batch, qc.ints, {qc.stage + (size_t)l * d.KVD, (int64_t)row, d.HD},
+              {qc.stage + ((size_t)qc.slots * d.L + l) * d.KVD, (int64_t)row, d.HD}, st);
+    q8_attend(v, batch, a, st);
+  };
+  if (m_->tc_all && !m_->tc) m_->tc = tc_model_build(m_->dm, m_->host_layers, m_->sms, st);
+  DEFER_CUDA(cudaEventRecord(ev_start_, st));
+  if (m_->tc_all) launch_step_tc_with(d, *m_->tc, bt, bs, m_->sms, m_->tc->work, st, attn);
+  else launch_step_phased_with(d, bt, bs, m_->sms, st, attn);
+  DEFER_CUDA(cudaEventRecord(ev_stop_, st));
+  int ctrl[8];
+  DEFER_CUDA(cudaMemcpyAsync(ctrl, d_ctrl_, sizeof(ctrl), cudaMemcpyDeviceToHost, st));
+  DEFER_CUDA(cudaStreamSynchronize(st));
+  float ms = 0.0f;
+  DEFER_CUDA(cudaEventElapsedTime(&ms, ev_start_, ev_stop_));
+  m_->t_device_ms += ms;
+  m_->t_runs += 1;
+  m_->t_launches += (uint64_t)(m_->tc_all ? launches_per_step_tc(d) : launches_per_step_phased(d));
+  m_->t_tokens += (uint64_t)n;
+  m_->t_bytes += kv_read + (double)m_->weight_bytes;
+  if (ctrl[0] == kStTimeout) fail(kDeviceTimeout, "a bounded wait of the token step timed out");
+  if (ctrl[0] != kStOk) fail(kModel, "the token step reported status " + std::to_string(ctrl[0]));
+  for (int b = 0; b < n; b++) qc.len[slots[b]]++;
+}
+
+void forward_q8(QuantCache* c, const uint32_t* slots, const uint32_t* tokens, size_t n, float* logits_out) {
+  const Model* m = c->model;
+  if (n > (size_t)c->slots) fail(kInvalidArgument, "more tokens than slots");
+  std::vector<char> named(c->slots, 0);
+  for (size_t i = 0; i < n; i++) {
+    need_slot(c, slots[i]);
+    if (named[slots[i]]) fail(kInvalidArgument, "slot " + std::to_string(slots[i]) + " is named twice");
+    named[slots[i]] = 1;
+    if (tokens[i] >= m->cfg.vocab_size) fail(kModel, "token id " + std::to_string(tokens[i]) + " out of range");
+    if (c->len[slots[i]] >= m->cfg.max_seq_len)
+      fail(kModel, "context length " + std::to_string(m->cfg.max_seq_len) + " exceeded");
+    if (c->len[slots[i]] >= (size_t)c->cap) fail(kModel, "cache capacity " + std::to_string(c->cap) + " exceeded");
+  }
+  if (n == 0) return;
+  // the runner's own attention is not used: chunk partials of one chunk
+  if (!c->runner || c->runner->capacity() < (int)n) c->runner.reset(new Runner(m, (int)n, kAttnChunk));
+  c->runner->step_q8(*c, slots, tokens, (int)n);
+  if (logits_out)
+    for (size_t i = 0; i < n; i++) c->runner->download_logits((int)i, logits_out + i * m->cfg.vocab_size);
 }
 
 // ----------------------------------------------------------- batch drivers

@@ -11,6 +11,7 @@
 #include "formats.h"
 #include "hostutil.h"
 #include "model.h"
+#include "q8.h"
 
 namespace defer {
 
@@ -39,6 +40,8 @@ struct SlotResult {
   std::vector<float> margins;
 };
 
+struct QuantCache;
+
 class Runner {
  public:
   Runner(const Model* m, int B, int max_cap);
@@ -53,6 +56,9 @@ class Runner {
   // Slot b's logits into slot db of `dst` (same model), on the model's stream.
   void copy_logits_to(int b, Runner& dst, int db) const;
   int last_steps() const { return last_steps_; }
+  // One token of n slots of an 8-bit cache (slot of the cache, token), their
+  // logits left in slots 0 .. n - 1 of the runner.
+  void step_q8(QuantCache& qc, const uint32_t* slots, const uint32_t* tokens, int n);
   // Runs whose programs never sample and fit one 128-slot MMA tile take the
   // tensor-core step (DEFER_B200_TC=0 keeps them on the CUDA cores).
   bool use_tc = false;
@@ -64,6 +70,7 @@ class Runner {
   int* tickets_ = nullptr;
   float* stats_ = nullptr;  // sampler block statistics, 5 arrays of [B][nblk]
   DSession* d_sess_ = nullptr;
+  DSession* d_staged_ = nullptr;  // the sessions of step_q8 with one-position caches
   DSlotState* d_state_ = nullptr;
   int* d_ctrl_ = nullptr;  // status, any_active[2], barrier counter
   uint32_t* d_scratch_ = nullptr;
@@ -74,6 +81,33 @@ class Runner {
   int last_steps_ = 0;
   cudaEvent_t ev_start_ = nullptr, ev_stop_ = nullptr;
 };
+
+// Key/value caches of `slots` sessions in 8 bits (q8.h), all layers in HBM,
+// with the buffers of a step over them.
+struct QuantCache {
+  const Model* model = nullptr;
+  int slots = 0, cap = 0, kind = 0;
+  std::vector<size_t> len;  // positions of each slot
+  unsigned char* mem = nullptr;
+  int* ints = nullptr;      // [3][slots]: positions, lengths and slots of a call
+  float* stage = nullptr;   // [2][slots][layers][kv_dim]: K and V rows of a step
+  float* ws = nullptr;      // workspace of the attention
+  size_t ws_bytes = 0;
+  std::unique_ptr<Runner> runner;
+  ~QuantCache();
+  Q8View view(int layer) const;
+};
+QuantCache* qcache_new(const Model* m, int slots, int cap, int kind);
+// KvCache::truncate of a slot: a shortened block that was closed is opened
+// again with the values that its codes stand for.
+void qcache_truncate(QuantCache* c, uint32_t slot, size_t n);
+// The whole of a KvCache into a slot, and a slot as a KvCache (values of the codes).
+void qcache_store(QuantCache* c, uint32_t slot, const KvCache* src);
+KvCache* qcache_load(const QuantCache* c, uint32_t slot);
+void qcache_download(const QuantCache* c, uint32_t slot, int layer, float* keys, float* values);
+// Model::forward (model.rs:376-520) of one token in each of n slots, attention
+// over the 8-bit cache; logits [n][vocab] to the host if non-null.
+void forward_q8(QuantCache* c, const uint32_t* slots, const uint32_t* tokens, size_t n, float* logits_out);
 
 // Whether runs use a persistent kernel (default) or one launch per phase
 // (DEFER_B200_PHASED=1).

@@ -265,6 +265,47 @@ static void phased_impl(const DModel& m, const DLayer* hl, const DBatch& bt0, in
   DEFER_CUDA(cudaGetLastError());
 }
 
+template <bool BF16, int G>
+static void phased_with_impl(const DModel& m, const DBatch& bt0, const DBatch& staged0, int sms, cudaStream_t st,
+                             const std::function<void(int)>& attn) {
+  const size_t sf = step_smem_floats(m, bt0.B, bt0.max_chunks);
+  const size_t smem = sf * sizeof(float);
+  DBatch bt = bt0, staged = staged0;
+  bt.smem_bytes = staged.smem_bytes = (unsigned)smem;
+  bt.parts = staged.parts = parts_for(m, bt.B, sms);
+  allow_smem(k_select<BF16>, smem);
+  allow_smem(k_qkv<BF16, G>, smem);
+  allow_smem(k_oproj<BF16, G>, smem);
+  allow_smem(k_gateup<BF16, G>, smem);
+  allow_smem(k_down<BF16, G>, smem);
+  allow_smem(k_head<BF16, G>, smem);
+  k_select<BF16><<<bt.B, kThreads, smem, st>>>(m, bt, 0);
+  for (int l = 0; l < m.L; l++) {
+    k_qkv<BF16, G><<<sms, kThreads, smem, st>>>(m, staged, l);
+    attn(l);
+    k_oproj<BF16, G><<<sms, kThreads, smem, st>>>(m, bt, l, (unsigned)sf);
+    k_gateup<BF16, G><<<sms, kThreads, smem, st>>>(m, bt, l);
+    k_down<BF16, G><<<sms, kThreads, smem, st>>>(m, bt, l, (unsigned)sf);
+  }
+  k_head<BF16, G><<<sms, kThreads, smem, st>>>(m, bt);
+  k_finalize<<<bt.B, kThreads, 0, st>>>(bt);
+  DEFER_CUDA(cudaGetLastError());
+}
+
+void launch_step_phased_with(const DModel& m, const DBatch& bt, const DBatch& staged, int sms, cudaStream_t st,
+                             const std::function<void(int)>& attn) {
+  const int G = group_for(m, bt.B);
+  auto go = [&](auto f32, auto bf16) { (m.bf16 ? bf16 : f32)(m, bt, staged, sms, st, attn); };
+  switch (G) {
+    case 1: go(phased_with_impl<false, 1>, phased_with_impl<true, 1>); break;
+    case 2: go(phased_with_impl<false, 2>, phased_with_impl<true, 2>); break;
+    case 4: go(phased_with_impl<false, 4>, phased_with_impl<true, 4>); break;
+    case 8: go(phased_with_impl<false, 8>, phased_with_impl<true, 8>); break;
+    case 16: go(phased_with_impl<false, 16>, phased_with_impl<true, 16>); break;
+    default: go(phased_with_impl<false, 32>, phased_with_impl<true, 32>); break;
+  }
+}
+
 int launches_per_step_phased(const DModel& m) { return 2 + 6 * m.L; }
 
 void launch_steps_phased(const DModel& m, const DLayer* host_layers, const DBatch& bt, int first_step, int nsteps,

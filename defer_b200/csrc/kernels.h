@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <functional>
+
 #include "device.cuh"
 
 namespace defer {
@@ -14,6 +16,12 @@ size_t step_smem_bytes(const DModel& m, int B, int max_chunks);
 void launch_steps_phased(const DModel& m, const DLayer* host_layers, const DBatch& bt, int first_step, int nsteps,
                          int sms, cudaStream_t st);
 int launches_per_step_phased(const DModel& m);
+// One step with one launch per phase and the caller's attention: attn(l)
+// launches layer l's between its QKV and O projections, from bt.q and the rows
+// that the QKV epilogue stored through `staged` (bt with other sessions) to
+// bt.att.
+void launch_step_phased_with(const DModel& m, const DBatch& bt, const DBatch& staged, int sms, cudaStream_t st,
+                             const std::function<void(int)>& attn);
 
 // All phases of up to `nsteps` steps in one cooperative persistent launch
 // (one CTA per SM, bounded grid barriers between phases).

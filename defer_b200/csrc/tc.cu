@@ -654,8 +654,10 @@ void tc_gemm(const unsigned char* A, const TcMatrix& w, float* Y, int splits, un
 
 size_t tc_y_floats(const TcMatrix& w, int splits) { return (size_t)splits * kTcM * w.ntile * kTcBN; }
 
-void launch_steps_tc(const DModel& m, const TcModel& tm, const DBatch& bt0, int nsteps, int sms, TcWork& wk,
-                     cudaStream_t st) {
+// `attn`: the attention of a step over another cache than bt's sessions',
+// whose new rows go through `staged`; null for the step's own.
+static void steps_tc(const DModel& m, const TcModel& tm, const DBatch& bt0, int nsteps, int sms, TcWork& wk,
+                     cudaStream_t st, const DBatch* staged, const std::function<void(int)>* attn) {
   if (bt0.B > kTcM) fail(kInvalidArgument, "tensor-core step: more than 128 slots");
   DBatch bt = bt0;
   const size_t smem = step_smem_bytes(m, bt.B, bt.max_chunks);
@@ -685,9 +687,13 @@ void launch_steps_tc(const DModel& m, const TcModel& tm, const DBatch& bt0, int 
       // the A operand of QKV is ready (the step's first prep, or the last
       // layer's residual)
       tc_gemm(wk.A, T.qkv, wk.Y, T.s_qkv, wk.tickets, bt.status, st, act);
-      k_tc_qkv_epi<<<ew, 256, 0, st>>>(m, bt, l, wk.Y, 1, T.qkv.ntile * kTcBN);
-      k_tc_attn<<<std::min(attn_units, sms * 8), kThreads, smem, st>>>(m, bt, l);
-      k_tc_combine<<<sms, kThreads, 0, st>>>(m, bt);
+      k_tc_qkv_epi<<<ew, 256, 0, st>>>(m, staged ? *staged : bt, l, wk.Y, 1, T.qkv.ntile * kTcBN);
+      if (attn) {
+        (*attn)(l);
+      } else {
+        k_tc_attn<<<std::min(attn_units, sms * 8), kThreads, smem, st>>>(m, bt, l);
+        k_tc_combine<<<sms, kThreads, 0, st>>>(m, bt);
+      }
       tc_prep(bt.att, nullptr, 0.0f, m.QD, bt.B, bt.st, wk.A, at, st, act);
       tc_gemm(wk.A, T.o, wk.Y, T.s_o, wk.tickets, bt.status, st, act);
       k_tc_resid_prep<<<kTcM, 256, 0, st>>>(m, bt, wk.Y, T.o.ntile * kTcBN, T.ffn_norm, nkb_h, wk.A, act, at);
@@ -705,6 +711,16 @@ void launch_steps_tc(const DModel& m, const TcModel& tm, const DBatch& bt0, int 
   }
   k_tc_finalize<<<bt.B, kThreads, 0, st>>>(bt);
   DEFER_CUDA(cudaGetLastError());
+}
+
+void launch_steps_tc(const DModel& m, const TcModel& tm, const DBatch& bt, int nsteps, int sms, TcWork& wk,
+                     cudaStream_t st) {
+  steps_tc(m, tm, bt, nsteps, sms, wk, st, nullptr, nullptr);
+}
+
+void launch_step_tc_with(const DModel& m, const TcModel& tm, const DBatch& bt, const DBatch& staged, int sms, TcWork& wk,
+                         cudaStream_t st, const std::function<void(int)>& attn) {
+  steps_tc(m, tm, bt, 1, sms, wk, st, &staged, &attn);
 }
 
 int launches_per_step_tc(const DModel& m) { return 5 + 11 * m.L; }

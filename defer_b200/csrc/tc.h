@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <cstddef>
+#include <functional>
 #include <vector>
 
 #include "device.cuh"
@@ -78,6 +79,11 @@ void tc_gemm(const unsigned char* A, const TcMatrix& w, float* Y, int splits, un
 void launch_steps_tc(const DModel& m, const TcModel& tm, const DBatch& bt, int nsteps, int sms, TcWork& wk,
                      cudaStream_t st);
 int launches_per_step_tc(const DModel& m);
+// One step whose attention the caller launches: attn(l), from bt.q and the
+// rows that the QKV epilogue stored through `staged` to bt.att (as
+// launch_step_phased_with).
+void launch_step_tc_with(const DModel& m, const TcModel& tm, const DBatch& bt, const DBatch& staged, int sms, TcWork& wk,
+                         cudaStream_t st, const std::function<void(int)>& attn);
 
 // Y [M][N] = X [M][K] . W [N][K]^T on the tensor cores with host buffers
 // (the check of the contraction itself; M <= 128).

@@ -353,6 +353,34 @@ DEFER_API int defer_q8_attend(const defer_q8_cache* c, const defer_q8_batch* b, 
 DEFER_API int defer_q8_attend_workspace(const defer_q8_cache* c, const defer_q8_batch* b, uint32_t max_len,
                                         uint32_t heads, size_t* bytes);
 
+/* A model's caches in 8 bits: `slots` sessions of up to `cap` positions (0:
+ * max_position_embeddings; rounded up to 16), every layer, the open blocks in
+ * fp32. For models whose head_dim is a multiple of 16 up to 256. */
+typedef struct defer_qcache defer_qcache;
+DEFER_API int defer_qcache_new(defer_model* m, uint32_t slots, uint32_t cap, int32_t kind, defer_qcache** out);
+DEFER_API void defer_qcache_free(defer_qcache* c);
+/* Positions of a slot (0 for a slot that does not exist). */
+DEFER_API size_t defer_qcache_len(const defer_qcache* c, uint32_t slot);
+/* Shortens a slot (as KvCache::truncate, src/model.rs:211-220). A block that
+ * was closed and is shortened is opened again with its codes' values. */
+DEFER_API int defer_qcache_truncate(defer_qcache* c, uint32_t slot, size_t n);
+/* A cache of the same model into a slot, whose contents it replaces, and a
+ * slot as a new cache holding the codes' values. */
+DEFER_API int defer_qcache_store(defer_qcache* c, uint32_t slot, const defer_cache* src);
+DEFER_API int defer_qcache_load(const defer_qcache* c, uint32_t slot, defer_cache** out);
+/* Keys and values of a slot's layer as defer_cache_download gives them. */
+DEFER_API int defer_qcache_download(const defer_qcache* c, uint32_t slot, uint32_t layer, float* keys, float* values);
+/* One layer's buffers, for defer_q8_append, _read and _attend. A call that
+ * writes them does not change the slots' lengths that the handle counts. */
+DEFER_API int defer_qcache_view(const defer_qcache* c, uint32_t layer, defer_q8_cache* out);
+/* Model::forward (src/model.rs:376-520) of tokens[i] in slot slots[i], i < n,
+ * all in one step: each slot's K and V rows are appended to the 8-bit cache
+ * and attention reads it; logits_out (NULL, or n * vocab_size floats) receives
+ * the logits. No slot may be named twice. The projections are those of the
+ * batched token loops; a slot's result does not depend on the other slots. */
+DEFER_API int defer_forward_q8(defer_model* m, defer_qcache* c, const uint32_t* slots, const uint32_t* tokens,
+                               size_t n, float* logits_out);
+
 #ifdef __cplusplus
 }
 #endif
