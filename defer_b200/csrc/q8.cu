@@ -24,16 +24,31 @@ namespace {
 
 constexpr float kQ8Tiny = 6.018531076210112e-36f;  // 2^-117
 
-// Code byte of t = x * r, and the value of a code byte.
+// Codes of four values times r. `odd`: the block holds a NaN (stored as 0) or
+// an infinity (stored as +-Q); else |x * r| rounds to Q at most. int8: adding
+// 3 * 2^22 leaves the rounded number in the low byte.
 template <int KIND>
-__device__ __forceinline__ uint32_t encode(float t) {
-  t = t == t ? t : 0.0f;
+__device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float x3, float r, bool odd) {
+  float t[4] = {__fmul_rn(x0, r), __fmul_rn(x1, r), __fmul_rn(x2, r), __fmul_rn(x3, r)};
+  if (odd) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      t[e] = t[e] == t[e] ? t[e] : 0.0f;
+      if (KIND == kQ8Int8) t[e] = fminf(fmaxf(t[e], -127.0f), 127.0f);
+    }
+  }
   if constexpr (KIND == kQ8Int8) {
-    return (uint32_t)__float2int_rn(fminf(fmaxf(t, -127.0f), 127.0f)) & 0xFFu;
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) u[e] = __float_as_uint(__fadd_rn(t[e], 12582912.0f));
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
   } else {
-    return (uint32_t)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[0], t[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[2], t[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
   }
 }
+// The value of a code byte.
 template <int KIND>
 __device__ __forceinline__ float decode(uint32_t byte) {
   if constexpr (KIND == kQ8Int8) {
@@ -43,6 +58,17 @@ __device__ __forceinline__ float decode(uint32_t byte) {
   }
 }
 
+// Unit of this warp: block `blk0` (of per_seq), head and K or V `h2`, sequence
+// `i`; 4 warps a CTA, and fewer than 2^31 units (grid_of).
+__device__ __forceinline__ bool unit_of(int n, int heads2, int per_seq, int& blk0, int& h2, int& i) {
+  const unsigned w = blockIdx.x * 4u + (threadIdx.x >> 5);
+  const unsigned a = w / (unsigned)per_seq;
+  blk0 = (int)(w - a * (unsigned)per_seq);
+  i = (int)(a / (unsigned)heads2);
+  h2 = (int)(a - (unsigned)i * (unsigned)heads2);
+  return i < n;
+}
+
 // ------------------------------------------------------------------ append
 // One warp per (sequence, head, K or V, block). It holds the block in
 // registers: 16 bytes of input a lane and step, so a step reads 512
@@ -50,18 +76,16 @@ __device__ __forceinline__ float decode(uint32_t byte) {
 // codes. The warp of a sequence's first block also stores the open block
 // (the tail): it is the only one that reads the old tail, and it does so
 // before it writes.
-template <int TYPE, int KIND, int HDMAX>
-__global__ void __launch_bounds__(128) k_q8_append(Q8View c, Q8Batch b, const int* __restrict__ pos, Q8Rows rk,
+template <int TYPE, int KIND, int HDMAX, bool EXACT>
+__global__ void __launch_bounds__(128, HDMAX <= 64 ? 10 : HDMAX <= 128 ? 7 : 4) k_q8_append(Q8View c, Q8Batch b, const int* __restrict__ pos, Q8Rows rk,
                                                    Q8Rows rv, int aligned, int per_seq) {
   using E = Elem<TYPE>;
   using T = typename E::T;
   constexpr int VEC = 16 / (int)sizeof(T);             // elements of one step and lane
   constexpr int STEPS = kQ8Block * HDMAX / VEC / 32;  // at the widest head
   const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int heads2 = 2 * c.kvh;
-  if (w >= (int64_t)b.n * heads2 * per_seq) return;
-  const int blk0 = (int)(w % per_seq), h2 = (int)(w / per_seq % heads2), i = (int)(w / per_seq / heads2);
+  int blk0, h2, i;
+  if (!unit_of(b.n, 2 * c.kvh, per_seq, blk0, h2, i)) return;
   const Seq s = seq_of(b, c.slots, i);
   if (s.slot < 0) return;
   const int p0 = __ldg(pos + i);
@@ -77,7 +101,7 @@ __global__ void __launch_bounds__(128) k_q8_append(Q8View c, Q8Batch b, const in
       return;
     }
   }
-  const int h = h2 >> 1, hd = c.hd;
+  const int h = h2 >> 1, hd = EXACT ? HDMAX : c.hd;
   const bool is_v = h2 & 1;
   const T* src = static_cast<const T*>(is_v ? rv.p : rk.p) + (size_t)h * (is_v ? rv.head : rk.head);
   const int64_t ts = is_v ? rv.token : rk.token;
@@ -98,6 +122,7 @@ __global__ void __launch_bounds__(128) k_q8_append(Q8View c, Q8Batch b, const in
   for (int blk = first + blk0; blk < open; blk += per_seq) {  // blocks that close
     __align__(16) T x[STEPS][VEC];
     float a = 0.0f;
+    bool odd = false;
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
       const int u = j * 32 + lane;
@@ -108,11 +133,14 @@ __global__ void __launch_bounds__(128) k_q8_append(Q8View c, Q8Batch b, const in
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
           const float f = fabsf(E::to(x[j][e]));
-          a = fmaxf(a, f <= FLT_MAX ? f : 0.0f);
+          const bool fine = f <= FLT_MAX;
+          odd |= !fine;
+          a = fmaxf(a, fine ? f : 0.0f);
         }
       }
     }
     a = warp_max_all(a);
+    odd = __any_sync(0xffffffffu, odd);
     const float sc = a < kQ8Tiny ? 0.0f : __fdiv_rn(a, KIND == kQ8Int8 ? 127.0f : 448.0f);
     const float rc = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
     if (lane == 0) scales[blk] = sc;
@@ -124,9 +152,7 @@ __global__ void __launch_bounds__(128) k_q8_append(Q8View c, Q8Batch b, const in
         uint32_t o[VEC / 4];
 #pragma unroll
         for (int e = 0; e < VEC; e += 4)
-          o[e / 4] = encode<KIND>(__fmul_rn(E::to(x[j][e]), rc)) | encode<KIND>(__fmul_rn(E::to(x[j][e + 1]), rc)) << 8 |
-                     encode<KIND>(__fmul_rn(E::to(x[j][e + 2]), rc)) << 16 |
-                     encode<KIND>(__fmul_rn(E::to(x[j][e + 3]), rc)) << 24;
+          o[e / 4] = encode4<KIND>(E::to(x[j][e]), E::to(x[j][e + 1]), E::to(x[j][e + 2]), E::to(x[j][e + 3]), rc, odd);
         if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(cb + (size_t)u * VEC) = o[0];
         else *reinterpret_cast<uint2*>(cb + (size_t)u * VEC) = make_uint2(o[0], o[1]);
       }
@@ -147,7 +173,7 @@ __global__ void __launch_bounds__(128) k_q8_append(Q8View c, Q8Batch b, const in
 // -------------------------------------------------------------------- read
 // One warp per (sequence, head, K or V, block); 16 bytes of output a lane
 // and step, stored past L1.
-template <int TYPE, int KIND>
+template <int TYPE, int KIND, int HD>
 __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __restrict__ lens,
                                                  const int* __restrict__ start, const int* __restrict__ slots,
                                                  int* status, int rows, Q8Out ok, Q8Out ov, int aligned,
@@ -156,10 +182,8 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
   using T = typename E::T;
   constexpr int VEC = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int heads2 = 2 * c.kvh;
-  if (w >= (int64_t)n * heads2 * per_seq) return;
-  const int blk0 = (int)(w % per_seq), h2 = (int)(w / per_seq % heads2), i = (int)(w / per_seq / heads2);
+  int blk0, h2, i;
+  if (!unit_of(n, 2 * c.kvh, per_seq, blk0, h2, i)) return;
   const int slot = slots ? __ldg(slots + i) : i;
   if (slot < 0) return;
   const int len = __ldg(lens + i), p0 = start ? __ldg(start + i) : 0;
@@ -170,7 +194,7 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
   const int p1 = (int)min((int64_t)len, (int64_t)p0 + rows);
   const int blk = p0 / kQ8Block + blk0;
   if ((int64_t)blk * kQ8Block >= p1) return;
-  const int h = h2 >> 1, hd = c.hd;
+  const int h = h2 >> 1, hd = HD ? HD : c.hd;
   const bool is_v = h2 & 1;
   const Q8Out& o = is_v ? ov : ok;
   T* dst = static_cast<T*>(o.p) + (int64_t)i * o.seq + (int64_t)h * o.head;
@@ -180,32 +204,41 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
   const bool open = blk == len / kQ8Block;
   const float sc = open ? 0.0f : (is_v ? c.vs : c.ks)[sh * (c.cap / kQ8Block) + blk];
   const int vrow = hd / VEC, vblk = kQ8Block * vrow;
-#pragma unroll 4
-  for (int u = lane; u < vblk; u += 32) {
-    const int r = u / vrow, d = (u - r * vrow) * VEC, p = blk * kQ8Block + r;
-    if (p < p0 || p >= p1) continue;
-    __align__(16) T x[VEC];
-    if (open) {
-      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(tail + r * hd + d);
-    } else {
-      uint32_t q[VEC / 4];
+  constexpr int PART = HD ? kQ8Block * HD / VEC / 32 : 1;  // steps whose loads are sent off together
+#pragma unroll 1
+  for (int u0 = lane; u0 < vblk; u0 += 32 * PART) {
+    uint32_t q[PART][VEC / 4];
+#pragma unroll
+    for (int j = 0; j < PART; j++) {
+      const size_t at = (size_t)(u0 + 32 * j) * VEC;
+      if (open) continue;
       if constexpr (VEC == 4) {
-        q[0] = __ldg(reinterpret_cast<const uint32_t*>(cb + (size_t)u * VEC));
+        q[j][0] = __ldcs(reinterpret_cast<const uint32_t*>(cb + at));
       } else {
-        const uint2 q2 = __ldg(reinterpret_cast<const uint2*>(cb + (size_t)u * VEC));
-        q[0] = q2.x;
-        q[1] = q2.y;
+        const uint2 q2 = __ldcs(reinterpret_cast<const uint2*>(cb + at));
+        q[j][0] = q2.x;
+        q[j][1] = q2.y;
       }
-#pragma unroll
-      for (int e = 0; e < VEC; e++)
-        x[e] = E::from(__fmul_rn(decode<KIND>(q[e / 4] >> (8 * (e & 3)) & 0xFFu), sc));
     }
-    T* y = dst + (int64_t)(p - p0) * o.token + d;
-    if (aligned) {
-      __stcs(reinterpret_cast<uint4*>(y), *reinterpret_cast<uint4*>(x));
-    } else {
 #pragma unroll
-      for (int e = 0; e < VEC; e++) y[e] = x[e];
+    for (int j = 0; j < PART; j++) {
+      const int u = u0 + 32 * j, r = u / vrow, d = (u - r * vrow) * VEC, p = blk * kQ8Block + r;
+      if (p < p0 || p >= p1) continue;
+      __align__(16) T x[VEC];
+      if (open) {
+        *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(tail + r * hd + d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+          x[e] = E::from(__fmul_rn(decode<KIND>(q[j][e / 4] >> (8 * (e & 3)) & 0xFFu), sc));
+      }
+      T* y = dst + (int64_t)(p - p0) * o.token + d;
+      if (aligned) {
+        __stcs(reinterpret_cast<uint4*>(y), *reinterpret_cast<uint4*>(x));
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) y[e] = x[e];
+      }
     }
   }
 }
@@ -268,14 +301,17 @@ constexpr size_t qs_smem() {
          + (size_t)(8 * NT) * (3 + 2 * kQsWarps) * 4;      // row factors, m and l of the CTA and of the warps
 }
 
-// Splits of a sequence with `closed` positions in closed blocks: of 4 units
-// or more up to 8 splits (a single short sequence is a matter of latency), of
-// 8 units or more beyond (a CTA's start and its merges cost about 5 steps).
+// Splits of a sequence of `rows` rows a key head with `closed` positions in
+// closed blocks. Up to 16 rows: of 4 units or more up to 8 splits (a single
+// short sequence is a matter of latency: 14 us instead of 16 for 1041 positions
+// of the 135M heads), of 8 units or more beyond (a CTA's start and its merges
+// cost about 5 steps). More rows are many CTAs anyway: of 8 units or more (512
+// rows over 2048 positions of the 135M heads: 43 us instead of 65).
 template <int HDP>
-__host__ __device__ __forceinline__ int qs_splits(int closed) {
+__host__ __device__ __forceinline__ int qs_splits(int closed, int64_t rows) {
   const int units = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT;
-  const int n = units < 64 ? units / 4 : units / 8;
-  return n < 1 ? 1 : units < 64 && n > kQsCluster ? kQsCluster : n > kQsMaxSplits ? kQsMaxSplits : n;
+  const int n = rows > 16 || units >= 64 ? units / 8 : units / 4 < kQsCluster ? units / 4 : kQsCluster;
+  return n < 1 ? 1 : n > kQsMaxSplits ? kQsMaxSplits : n;
 }
 
 // Position (of 8) that row r of the score product stands for: the positions of
@@ -402,7 +438,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
     return;
   }
   const int hd = EXACT ? HDP : c.hd, closed = len & ~(kQ8Block - 1);
-  const int splits = min(qs_splits<HDP>(closed), groups * csize);
+  const int splits = min(qs_splits<HDP>(closed, R), groups * csize);
   const int split = group * kQsCluster + rank, ns = min(splits - group * kQsCluster, csize);  // ns: of the cluster
   if (rank >= ns) return;  // cluster barriers wait for the CTAs that are left
   const size_t sh = (size_t)s.slot * c.kvh + kvh;
@@ -862,7 +898,8 @@ __global__ void __launch_bounds__(128) k_q8_merge(Q8View c, Q8Batch b, Q8Attend 
   const int len = __ldg(a.lens + i);
   if (s.slot < 0 || token < s.row0 || token >= s.row0 + s.nrow || len < 0 || len > c.cap) return;
   if (a.tiled && s.nrow * (a.heads / c.kvh) > kQ8FewRows) return;
-  const int splits = min(qs_splits<HDP>(len & ~(kQ8Block - 1)), groups * kQsCluster);
+  const int splits =
+      min(qs_splits<HDP>(len & ~(kQ8Block - 1), (int64_t)s.nrow * (a.heads / c.kvh)), groups * kQsCluster);
   if (splits <= kQsCluster) return;
   const int n = (splits + kQsCluster - 1) / kQsCluster;
   const float* y = a.ws + (size_t)w * groups * (c.hd + 4);
@@ -895,9 +932,8 @@ bool aligned16(const void* p, int64_t s0, int64_t s1, int64_t s2, int esize) {
 int esize_of(int type) { return type == kQ8F32 ? 4 : 2; }
 
 unsigned grid_of(int64_t warps) {
-  const int64_t g = (warps + 3) / 4;
-  if (g > INT32_MAX) fail(kInvalidArgument, "8-bit cache: too many sequences and heads in one call");
-  return (unsigned)g;
+  if (warps >= INT32_MAX) fail(kInvalidArgument, "8-bit cache: too many sequences, heads and blocks in one call");
+  return (unsigned)((warps + 3) / 4);
 }
 
 // f(type constant, kind constant)
@@ -927,9 +963,11 @@ void q8_append(const Q8View& c, const Q8Batch& b, const int* pos, const Q8Rows& 
   const unsigned grid = grid_of((int64_t)b.n * 2 * c.kvh * per_seq);
   dispatch(c, [&](auto type, auto kind) {
     constexpr int TY = decltype(type)::value, KI = decltype(kind)::value;
-    if (c.hd <= 64) k_q8_append<TY, KI, 64><<<grid, 128, 0, st>>>(c, b, pos, k, v, al, per_seq);
-    else if (c.hd <= 128) k_q8_append<TY, KI, 128><<<grid, 128, 0, st>>>(c, b, pos, k, v, al, per_seq);
-    else k_q8_append<TY, KI, 256><<<grid, 128, 0, st>>>(c, b, pos, k, v, al, per_seq);
+    auto kern = c.hd == 64    ? k_q8_append<TY, KI, 64, true>
+                : c.hd == 128 ? k_q8_append<TY, KI, 128, true>
+                : c.hd <= 128 ? k_q8_append<TY, KI, 128, false>
+                              : k_q8_append<TY, KI, 256, false>;
+    kern<<<grid, 128, 0, st>>>(c, b, pos, k, v, al, per_seq);
   });
   DEFER_CUDA(cudaGetLastError());
 }
@@ -943,8 +981,9 @@ void q8_read(const Q8View& c, int n, const int* lens, const int* start, const in
   const int per_seq = start ? (most + 2 * kQ8Block - 2) / kQ8Block : (most + kQ8Block - 1) / kQ8Block;
   const unsigned grid = grid_of((int64_t)n * 2 * c.kvh * per_seq);
   dispatch(c, [&](auto type, auto kind) {
-    k_q8_read<decltype(type)::value, decltype(kind)::value>
-        <<<grid, 128, 0, st>>>(c, n, lens, start, slots, status, rows, k, v, al, per_seq);
+    constexpr int TY = decltype(type)::value, KI = decltype(kind)::value;
+    auto kern = c.hd == 64 ? k_q8_read<TY, KI, 64> : c.hd == 128 ? k_q8_read<TY, KI, 128> : k_q8_read<TY, KI, 0>;
+    kern<<<grid, 128, 0, st>>>(c, n, lens, start, slots, status, rows, k, v, al, per_seq);
   });
   DEFER_CUDA(cudaGetLastError());
 }
@@ -969,9 +1008,11 @@ void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream
   if (first_on_device(attr)) {
     DEFER_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
-  const int64_t rows = (int64_t)std::max(b.max_q, 1) * (a.heads / c.kvh);
+  int64_t rows = (int64_t)std::max(b.max_q, 1) * (a.heads / c.kvh);
+  if (a.tiled) rows = std::min<int64_t>(rows, kQ8FewRows);
   const int64_t tiles = std::min<int64_t>((rows + 8 * NT - 1) / (8 * NT), 65535 / c.kvh);
-  const int splits = qs_splits<HDP>(a.max_len / kQ8Block * kQ8Block);  // of the longest sequence
+  // of the longest sequence, which with q_start may have few rows
+  const int splits = qs_splits<HDP>(a.max_len / kQ8Block * kQ8Block, b.q_start ? 1 : rows);
   const int groups = (splits + kQsCluster - 1) / kQsCluster;
   int cl = 1;  // a power of two that holds its splits
   while (cl < std::min(splits, kQsCluster)) cl *= 2;
@@ -995,8 +1036,11 @@ void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream
 size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a) {
   if (!b.q_start && q8_tiles(c, b, a)) return 0;
   const int closed = a.max_len / kQ8Block * kQ8Block;
-  const int splits = c.hd <= 32 ? qs_splits<32>(closed) : c.hd <= 64 ? qs_splits<64>(closed)
-                     : c.hd <= 128 ? qs_splits<128>(closed) : qs_splits<256>(closed);
+  const int64_t rows = b.q_start ? 1 : (int64_t)std::max(b.max_q, 1) * (a.heads / c.kvh);
+  const int splits = c.hd <= 32    ? qs_splits<32>(closed, rows)
+                     : c.hd <= 64  ? qs_splits<64>(closed, rows)
+                     : c.hd <= 128 ? qs_splits<128>(closed, rows)
+                                   : qs_splits<256>(closed, rows);
   if (splits <= kQsCluster) return 0;
   return (size_t)b.tokens * a.heads * ((splits + kQsCluster - 1) / kQsCluster) * (c.hd + 4) * sizeof(float);
 }

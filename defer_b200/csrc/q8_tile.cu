@@ -16,10 +16,10 @@
 // Work: a CTA takes two tiles of 128 rows (rows of the heads that share a key
 // head, token after token), so that a converted block of 128 positions feeds
 // two products and one tile's softmax runs beside the other's products. Warps
-// 0-3 and 4-7: softmax of one tile each, a row a thread; warps 8-11 turn the
-// codes of K and V into fp16 in shared memory (two stages each, no-swizzle
-// core matrices: K read K-major, V MN-major, so both are stored alike and
-// nothing is transposed); warp 12 issues the products. Tensor memory holds two
+// 0-3 and 4-7: softmax of one tile each, a row a thread; warps 8-11 and 12-15
+// turn the codes of K and of V into fp16 in shared memory (two stages each,
+// no-swizzle core matrices: K read K-major, V MN-major, so both are stored
+// alike and nothing is transposed); warp 16 issues the products. Tensor memory holds two
 // score tiles and two outputs (512 columns); the weights overwrite the scores
 // they came from and are the A operand from there. The order of the products
 // (PV of tile 0, scores of tile 0 of the next block, the same of tile 1) keeps
@@ -40,7 +40,7 @@ namespace {
 
 constexpr int kQtM = 128;          // rows of a tile
 constexpr int kQtN = 128;          // positions of a block
-constexpr int kQtThreads = 13 * 32;
+constexpr int kQtThreads = 17 * 32;
 constexpr int kQtSlots = 4;        // ring of scales and masks
 constexpr unsigned long long kQtWaitNs = 2000000000ull;
 
@@ -62,10 +62,9 @@ struct QtShared {
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
   uint32_t tmem;
   int failed;
-  float open_k, open_v;  // scales of the open block
-  int open_odd;          // its values hold a NaN or an infinity
-  float red[2][4];
-  int red_odd[4];
+  int open_odd;          // the open block's values hold a NaN or an infinity
+  float red[2][2][4];
+  int red_odd[2][4];
   float fac[2 * kQtM];   // row factors
 };
 
@@ -142,14 +141,18 @@ __device__ __forceinline__ void qt_proxy() { asm volatile("fence.proxy.async.sha
 
 #define QT_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
 #define QT_W8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
-// 32 columns of the warp's 32 lanes, complete on return.
+// 32 columns of the warp's 32 lanes; the registers hold them after tm_wait.
 __device__ __forceinline__ void tm_ld32(uint32_t (&v)[32], uint32_t a) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : QT_R8(v, 0), QT_R8(v, 8), QT_R8(v, 16), QT_R8(v, 24)
       : "r"(a)
       : "memory");
+}
+#define QT_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+__device__ __forceinline__ void tm_wait(uint32_t (&v)[32]) {  // every load of the thread; v is used only behind it
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : QT_RW8(v, 0), QT_RW8(v, 8), QT_RW8(v, 16), QT_RW8(v, 24) : : "memory");
 }
 __device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t (&v)[32]) {
   asm volatile(
@@ -165,6 +168,36 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&v)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two fp32 numbers in one register pair, and the operations on both at once.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void f2_get(uint64_t d, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
@@ -213,7 +246,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     S.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -322,29 +355,34 @@ __global__ void __launch_bounds__(kQtThreads, 1)
           all &= show[j] == 0xffffffffu;
         }
         all = __all_sync(0xffffffffu, all);
+        // A row's scores of 32 positions from tensor memory; hidden ones are -inf.
+        auto hide32 = [&](uint32_t (&v)[32], int j) {
+          if (all) return;
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (!(show[j] >> e & 1)) v[e] = 0xff800000u;
+        };
+        // Scale of a block's scores: never 0, which would turn -inf into NaN;
+        // scores (below 2^30) times this least one are 0 to every bit that counts.
+        auto scale_of = [&](int g) { return fmaxf(sc.ks[g] * fs, 1.0e-36f); };
+        uint32_t v[2][32];  // one part is worked on while the next one comes
         // ---- the largest score with its value scale
         float mx = -INFINITY;
-#pragma unroll 1
-        for (int j = 0; j < 4; j++) {
-          uint32_t v[32];
-          tm_ld32(v, ts + j * 32);
-          if (!all) {
-            uint32_t w = show[0];
-            if (j == 1) w = show[1];
-            if (j == 2) w = show[2];
-            if (j == 3) w = show[3];
+        tm_ld32(v[0], ts);
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              if (!(w >> e & 1)) v[e] = 0xff800000u;
-          }
+        for (int j = 0; j < 4; j++) {
+          uint32_t(&w)[32] = v[j & 1];
+          tm_wait(w);
+          if (j < 3) tm_ld32(v[(j + 1) & 1], ts + (j + 1) * 32);
+          else tm_ld32(v[0], ts);  // the second pass begins
+          hide32(w, j);
 #pragma unroll
           for (int g = 0; g < 2; g++) {
-            float y = __uint_as_float(v[g * 16]);
+            float y = __uint_as_float(w[g * 16]);
 #pragma unroll
-            for (int e = 1; e < 16; e++) y = fmaxf(y, __uint_as_float(v[g * 16 + e]));
-            const float cs = sc.ks[2 * j + g] * fs;
-            // a block whose scores are all zero by its scale: 0 x -inf is no score
-            mx = fmaxf(mx, (y == -INFINITY ? y : y * cs) + sc.lam[2 * j + g]);
+            for (int e = 1; e < 15; e += 2) y = max3(y, __uint_as_float(w[g * 16 + e]), __uint_as_float(w[g * 16 + e + 1]));
+            y = fmaxf(y, __uint_as_float(w[g * 16 + 15]));
+            mx = fmaxf(mx, fmaf(y, scale_of(2 * j + g), sc.lam[2 * j + g]));
           }
         }
         // ---- move the reference when it has fallen far behind
@@ -358,49 +396,47 @@ __global__ void __launch_bounds__(kQtThreads, 1)
             l *= al;
 #pragma unroll 1
             for (int j = 0; j < HDT / 32; j++) {
-              uint32_t v[32];
-              tm_ld32(v, to + j * 32);
+              uint32_t w[32];
+              tm_ld32(w, to + j * 32);
+              tm_wait(w);
 #pragma unroll
-              for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * al);
-              tm_st32(to + j * 32, v);
+              for (int e = 0; e < 32; e++) w[e] = __float_as_uint(__uint_as_float(w[e]) * al);
+              tm_st32(to + j * 32, w);
             }
             tm_wait_st();
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
         // ---- weights over the scores
-#pragma unroll 1
-        for (int j = 0; j < 4; j++) {
-          uint32_t v[32], p[16];
-          tm_ld32(v, ts + j * 32);
-          if (!all) {
-            uint32_t w = show[0];
-            if (j == 1) w = show[1];
-            if (j == 2) w = show[2];
-            if (j == 3) w = show[3];
+        const uint64_t nref = f2(-ref, -ref);
+        uint64_t l2 = f2(0.0f, 0.0f);
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              if (!(w >> e & 1)) v[e] = 0xff800000u;
-          }
+        for (int j = 0; j < 4; j++) {
+          uint32_t(&w)[32] = v[j & 1];
+          tm_wait(w);
+          if (j < 3) tm_ld32(v[(j + 1) & 1], ts + (j + 1) * 32);
+          hide32(w, j);
+          uint32_t p[16];
 #pragma unroll
           for (int g = 0; g < 2; g++) {
-            const float cs = sc.ks[2 * j + g] * fs, vs = sc.vs64[2 * j + g];
-            float l0 = 0.0f, l1 = 0.0f;
+            const float cs = scale_of(2 * j + g), vs = sc.vs64[2 * j + g];
+            const uint64_t cs2 = f2(cs, cs), vs2 = f2(vs, vs);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              float p0 = ex2(fmaf(__uint_as_float(v[g * 16 + e]), cs, -ref));
-              float p1 = ex2(fmaf(__uint_as_float(v[g * 16 + e + 1]), cs, -ref));
-              if (cs == 0.0f) {  // hidden positions again: 0 x -inf
-                p0 = v[g * 16 + e] == 0xff800000u ? 0.0f : p0;
-                p1 = v[g * 16 + e + 1] == 0xff800000u ? 0.0f : p1;
-              }
-              l0 += p0;
-              l1 += p1;
-              p[g * 8 + e / 2] = h2_bits(__floats2half2_rn(p0 * vs, p1 * vs));
+              float p0, p1;
+              f2_get(f2_fma(f2(__uint_as_float(w[g * 16 + e]), __uint_as_float(w[g * 16 + e + 1])), cs2, nref), p0, p1);
+              const uint64_t pp = f2(ex2(p0), ex2(p1));
+              l2 = f2_add(l2, pp);
+              f2_get(f2_mul(pp, vs2), p0, p1);
+              p[g * 8 + e / 2] = h2_bits(__floats2half2_rn(p0, p1));
             }
-            l += l0 + l1;
           }
           tm_st16(ts + j * 16, p);
+        }
+        {
+          float l0, l1;
+          f2_get(l2, l0, l1);
+          l += l0 + l1;
         }
         tm_wait_st();
         qt_before();
@@ -418,6 +454,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         __syncwarp();
         if (ok && nb) {
           tm_ld32(v, to + j * 32);
+          tm_wait(v);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e++) v[e] = ok ? 0u : 0x7fc00000u;
@@ -463,14 +500,16 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       }
       qt_before();  // this item's output is read before the next item's products
     }
-  } else if (wg == 2) {
-    // ------------------------------- codes to fp16 operands, scales and masks
-    const int ct = tid - 256, cw = ct >> 5, r8 = lane & 7, c4 = lane >> 3;
+  } else if (wg < 4) {
+    // ------------- codes to fp16 operands (K and V by four warps each), scales and masks (K's)
+    const bool is_v = wg == 3;
+    const int ct = tid & 127, cw = ct >> 5, r8 = lane & 7, c4 = lane >> 3;
     constexpr int SETS = HDT / 64;  // sets of four 16-code chunks of a row
-    const unsigned char* kc = c.kc + sh * c.cap * hd;
-    const unsigned char* vc = c.vc + sh * c.cap * hd;
+    const unsigned char* codes = (is_v ? c.vc : c.kc) + sh * c.cap * hd;
+    const T* tail = is_v ? vt : kt;
     const float* ksc = c.ks + sh * (c.cap / kQ8Block);
     const float* vsc = c.vs + sh * (c.cap / kQ8Block);
+    float open_k, open_v;
     {  // the open block's power-of-two scales: its largest finite element that is not hidden becomes [2^6, 2^7)
       float ak = 0.0f, av = 0.0f;
       bool odd = false;
@@ -485,120 +524,115 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       av = warp_max_all(av);
       odd = __any_sync(0xffffffffu, odd);
       if (lane == 0) {
-        S.red[0][cw] = ak;
-        S.red[1][cw] = av;
-        S.red_odd[cw] = odd;
+        S.red[is_v][0][cw] = ak;
+        S.red[is_v][1][cw] = av;
+        S.red_odd[is_v][cw] = odd;
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const float mk = fmaxf(fmaxf(S.red[0][0], S.red[0][1]), fmaxf(S.red[0][2], S.red[0][3]));
-      const float mv = fmaxf(fmaxf(S.red[1][0], S.red[1][1]), fmaxf(S.red[1][2], S.red[1][3]));
-      if (ct == 0) {
-        // exponents from -96: smaller blocks keep fewer than their own bits
-        S.open_k = mk > 0.0f ? exp2i(max(exponent_of(mk), -96) - 6) : 1.0f;
-        S.open_v = mv > 0.0f ? exp2i(max(exponent_of(mv), -96) - 6) : 1.0f;
-        S.open_odd = S.red_odd[0] | S.red_odd[1] | S.red_odd[2] | S.red_odd[3];
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + (int)is_v) : "memory");
+      const float* rk = S.red[is_v][0];
+      const float* rv = S.red[is_v][1];
+      const float mk = fmaxf(fmaxf(rk[0], rk[1]), fmaxf(rk[2], rk[3]));
+      const float mv = fmaxf(fmaxf(rv[0], rv[1]), fmaxf(rv[2], rv[3]));
+      // exponents from -96: smaller blocks keep fewer than their own bits
+      open_k = mk > 0.0f ? exp2i(max(exponent_of(mk), -96) - 6) : 1.0f;
+      open_v = mv > 0.0f ? exp2i(max(exponent_of(mv), -96) - 6) : 1.0f;
+      const int* ro = S.red_odd[is_v];
+      if (ct == 0 && !is_v) S.open_odd = ro[0] | ro[1] | ro[2] | ro[3];
     }
-    const float open_k = S.open_k, open_v = S.open_v;
-    const float up_k = 1.0f / open_k, up_v = 1.0f / open_v;
-    uint4 rk[4 * SETS], rv[4 * SETS];
-    auto load = [&](uint4 (&x)[4 * SETS], const unsigned char* src, int t) {
+    const float up = 1.0f / (is_v ? open_v : open_k);
+    uint4 x[4 * SETS];
+    auto load = [&](int t) {
 #pragma unroll
       for (int g = 0; g < 4; g++)
 #pragma unroll
         for (int z = 0; z < SETS; z++) {
           const int p = t * kQtN + (cw + 4 * g) * 8 + r8, ch = z * 4 + c4;
           x[g * SETS + z] = p < closed && ch * 16 < hd
-                                ? __ldg(reinterpret_cast<const uint4*>(src + (size_t)p * hd + ch * 16))
+                                ? __ldg(reinterpret_cast<const uint4*>(codes + (size_t)p * hd + ch * 16))
                                 : make_uint4(0, 0, 0, 0);
         }
     };
-    auto store = [&](const uint4 (&x)[4 * SETS], unsigned char* dst, int t, const T* tail, float up, bool values) {
+    auto store = [&](unsigned char* dst, int t) {
 #pragma unroll
       for (int g = 0; g < 4; g++)
 #pragma unroll
         for (int z = 0; z < SETS; z++) {
-          const int p = t * kQtN + (cw + 4 * g) * 8 + r8, ch = z * 4 + c4;
+          const int ch = z * 4 + c4;
           unsigned char* d = dst + (cw + 4 * g) * GROUP + ch * 256 + r8 * 16;
           uint32_t o[8];
-          if (p >= closed && p < len && ch * 16 < hd) {
-            const T* y = tail + (p - closed) * hd + ch * 16;
-            const bool hid = hide && hide[p];
+          const uint4 w = x[g * SETS + z];
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-              float y0 = E::to(y[2 * e]), y1 = E::to(y[2 * e + 1]);
-              if (values) {  // a weight of 0 times one of these would spread; they are added at the end
-                y0 = fabsf(y0) <= FLT_MAX ? y0 : 0.0f;
-                y1 = fabsf(y1) <= FLT_MAX ? y1 : 0.0f;
-              }
-              o[e] = hid ? 0u : h2_bits(__floats2half2_rn(y0 * up, y1 * up));
-            }
-          } else {
-            const uint4 w = x[g * SETS + z];
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const uint32_t u = flip<KIND>(ww[e]);
-              o[2 * e] = halves<KIND, false>(u);
-              o[2 * e + 1] = halves<KIND, true>(u);
-            }
+          for (int e = 0; e < 4; e++) {
+            const uint32_t u = flip<KIND>(ww[e]);
+            o[2 * e] = halves<KIND, false>(u);
+            o[2 * e + 1] = halves<KIND, true>(u);
           }
           *reinterpret_cast<uint4*>(d) = make_uint4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<uint4*>(d + 128) = make_uint4(o[4], o[5], o[6], o[7]);
         }
+      if ((t + 1) * kQtN <= closed || t * kQtN >= len) return;
+      // the open block's tokens, over the zeros that the warps have put in their place
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + (int)is_v) : "memory");
+#pragma unroll 1
+      for (int u = ct; u < (len - closed) * (hd / 8); u += 128) {
+        const int p = closed + u / (hd / 8) - t * kQtN, d8 = u % (hd / 8);
+        if (p < 0 || p >= kQtN) continue;
+        const T* y = tail + (u / (hd / 8)) * hd + d8 * 8;
+        const bool hid = hide && hide[t * kQtN + p];
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float y0 = E::to(y[2 * e]), y1 = E::to(y[2 * e + 1]);
+          if (is_v) {  // a weight of 0 times one of these would spread; they are added at the end
+            y0 = fabsf(y0) <= FLT_MAX ? y0 : 0.0f;
+            y1 = fabsf(y1) <= FLT_MAX ? y1 : 0.0f;
+          }
+          o[e] = hid ? 0u : h2_bits(__floats2half2_rn(y0 * up, y1 * up));
+        }
+        *reinterpret_cast<uint4*>(dst + (p >> 3) * GROUP + d8 * 128 + (p & 7) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
     };
     unsigned n = 0;  // blocks of the CTA
     bool ok = true;
     for (int item = first; item < items && ok; item += tiles) {
       const int x0 = item * per_item, x_end = min(x0 + per_item, R);
       const int nb = max(blocks_to(min(x0 + kQtM, x_end) - 1), blocks_to(x_end - 1));
-      if (nb) {
-        load(rk, kc, 0);
-        load(rv, vc, 0);
-      }
+      if (nb) load(0);
       for (int t = 0; t < nb; t++, n++) {
         const unsigned st = n & 1, ph = (n >> 1) & 1;
-        // ---- scales and masks (the slot's last readers are behind: their block's products are done)
-        QtScales& sc = S.sc[n % kQtSlots];
-        const int p = t * kQtN + ct;
-        const uint32_t show = __ballot_sync(0xffffffffu, p < len && !(hide && hide[p]));
-        if (lane == 0) sc.show[cw] = show;
-        if (ct < kQtN / kQ8Block) {
-          const int p0 = t * kQtN + ct * kQ8Block;
-          float ks = 0.0f, vs = 0.0f;
-          if (p0 < closed) {
-            ks = __ldg(ksc + p0 / kQ8Block);
-            vs = __ldg(vsc + p0 / kQ8Block);
-          } else if (p0 < len) {
-            ks = open_k;
-            vs = open_v;
+        if (!is_v) {
+          // scales and masks; the slot's last readers are behind: k_empty of
+          // block n - 3 came after the products with block n - 4's weights
+          QtScales& sc = S.sc[n % kQtSlots];
+          const int p = t * kQtN + ct;
+          const uint32_t show = __ballot_sync(0xffffffffu, p < len && !(hide && hide[p]));
+          if (lane == 0) sc.show[cw] = show;
+          if (ct < kQtN / kQ8Block) {
+            const int p0 = t * kQtN + ct * kQ8Block;
+            float ks = 0.0f, vs = 0.0f;
+            if (p0 < closed) {
+              ks = __ldg(ksc + p0 / kQ8Block);
+              vs = __ldg(vsc + p0 / kQ8Block);
+            } else if (p0 < len) {
+              ks = open_k;
+              vs = open_v;
+            }
+            sc.ks[ct] = ks;
+            sc.vs64[ct] = vs * 64.0f;
+            sc.lam[ct] = scale_exponent(vs);
           }
-          sc.ks[ct] = ks;
-          sc.vs64[ct] = vs * 64.0f;
-          sc.lam[ct] = scale_exponent(vs);
+          qb_arrive(&S.sc_full[n % kQtSlots]);
         }
-        qb_arrive(&S.sc_full[n % kQtSlots]);
-        // ---- K
-        if (n >= 2) ok = qb_wait(&S.k_empty[st], ph ^ 1, failed);
+        if (n >= 2) ok = qb_wait(is_v ? &S.v_empty[st] : &S.k_empty[st], ph ^ 1, failed);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
-        store(rk, S.k[st], t, kt, up_k, false);
+        store(is_v ? S.v[st] : S.k[st], t);
         qt_proxy();
-        qb_arrive(&S.k_full[st]);
-        if (t + 1 < nb) load(rk, kc, t + 1);
-        // ---- V
-        if (n >= 2) ok = qb_wait(&S.v_empty[st], ph ^ 1, failed);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        store(rv, S.v[st], t, vt, up_v, true);
-        qt_proxy();
-        qb_arrive(&S.v_full[st]);
-        if (t + 1 < nb) load(rv, vc, t + 1);
+        qb_arrive(is_v ? &S.v_full[st] : &S.k_full[st]);
+        if (t + 1 < nb) load(t + 1);
       }
     }
   } else if (lane == 0) {
@@ -666,7 +700,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   }
   qt_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     qt_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
   }
