@@ -420,13 +420,17 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
   float* wl = wm + kQsWarps * ROWS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, cq = lane & 3;
   const int csize = (int)cluster_size(), rank = (int)cluster_rank();
-  const int i = (int)((unsigned)blockIdx.x / (unsigned)(csize * groups));
-  const int group = (int)((unsigned)blockIdx.x / (unsigned)csize) - i * groups;
-  const int kvh = (int)((unsigned)blockIdx.y / (unsigned)tiles);
+  // clusters are powers of two; the usual call has one group and one tile
+  const int cluster = (int)(blockIdx.x >> (31 - __clz(csize)));
+  const int i = groups == 1 ? cluster : (int)((unsigned)cluster / (unsigned)groups), group = cluster - i * groups;
+  const int kvh = tiles == 1 ? (int)blockIdx.y : (int)(blockIdx.y / (unsigned)tiles);
   int len = __ldg(a.lens + i);
   const Seq s = seq_of(b, c.slots, i);
-  const int G = a.heads / c.kvh, R = s.nrow * G;
+  const int G = a.group, R = s.nrow * G;
   if (s.slot == kSeqSkip || R == 0) return;
+  // x / G of a row x by a product with 2^32 / G rounded up: exact while x * G < 2^32
+  const bool small = R < 1 << 20 && G <= 4096;
+  auto token_of = [&](int x) { return G == 1 ? x : small ? (int)__umulhi((unsigned)x, a.group_inv) : x / G; };
   if (s.slot == kSeqBad) len = -1;
   if (a.tiled && R > kQ8FewRows) return;
   T* const out0 = static_cast<T*>(const_cast<void*>(a.out.p));
@@ -454,10 +458,13 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
     const int x0 = tile * ROWS;
     const int jlast = min(x0 + ROWS, R) - 1;
     // positions that the tile's last row sees bound the work of the tile
-    const int most = a.causal ? min(len, len - (s.nrow - 1 - jlast / G)) : len;
-    const int least = a.causal ? len - (s.nrow - 1 - x0 / G) : len;  // the first row's
-    const int u0 = (int)((unsigned)(units * split) / (unsigned)splits);
-    const int u1 = (int)((unsigned)(units * (split + 1)) / (unsigned)splits);
+    const int most = a.causal ? min(len, len - (s.nrow - 1 - token_of(jlast))) : len;
+    const int least = a.causal ? len - (s.nrow - 1 - token_of(x0)) : len;  // the first row's
+    int u0 = 0, u1 = units;
+    if (splits > 1) {
+      u0 = (int)((unsigned)(units * split) / (unsigned)splits);
+      u1 = (int)((unsigned)(units * (split + 1)) / (unsigned)splits);
+    }
     const int t_end = min(min(closed, most), u1 * S::UNIT);
     const int t_first = u0 * S::UNIT + warp * S::TS;
     const int steps = t_end > t_first ? (t_end - t_first + S::UNIT - 1) / S::UNIT : 0;
@@ -542,8 +549,9 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
     // q rows of the tile as score operands, a row a warp
     for (int x = warp; x < ROWS; x += kQsWarps) {
       const bool on = x0 + x < R;
-      const T* q = static_cast<const T*>(a.q.p) + (int64_t)(s.row0 + (x0 + x) / G) * a.q.token +
-                   (int64_t)(kvh * G + (x0 + x) % G) * a.q.head;
+      const int tok = token_of(x0 + x);
+      const T* q = static_cast<const T*>(a.q.p) + (int64_t)(s.row0 + tok) * a.q.token +
+                   (int64_t)(kvh * G + x0 + x - tok * G) * a.q.head;
       float v[HDP / 32], mx = 0.0f;
 #pragma unroll
       for (int e = 0; e < HDP / 32; e++) {
@@ -588,7 +596,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
         m[n][e] = -INFINITY;
         l[n][e] = 0.0f;
         f[n][e] = fac[x];
-        seen[n][e] = x0 + x >= R ? 0 : a.causal ? len - (s.nrow - 1 - (x0 + x) / G) : len;
+        seen[n][e] = x0 + x >= R ? 0 : a.causal ? len - (s.nrow - 1 - token_of(x0 + x)) : len;
       }
 
     for (int it = 0; it < steps; it++) {
@@ -712,66 +720,119 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
     cp_join();
     __syncwarp();
 
-    // ---- the open block
-    {
+    // ---- the open block: the scores of the warp's tokens, one move of the
+    // running maximum for all of them, then their values
+    if (n_open) {
       const T* kb = reinterpret_cast<const T*>(wo);
       const T* vb = kb + OPEN * hd + r * (HDP / 8);
-      for (int y = 0; y < n_open; y++) {
-        const int t = closed + warp + y * kQsWarps;
-        if (hide && hide[t]) continue;
-        const T *kr = kb + y * hd, *vr = vb + y * hd;
-        float vmax = 0.0f;  // of the token's values: the same part as a block's scale
+      auto quad = [](float (&f)[4], const T* p) {  // 4 elements, 8 or 16 bytes
+        __align__(16) T x[4];
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(p);
+        else *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(p);
 #pragma unroll
-        for (int d = 0; d < HDP / 8; d++)
-          if (r * (HDP / 8) + d < hd) vmax = fmaxf(vmax, fabsf(E::to(vr[d])));
-        const float lam = scale_exponent(warp_max_all(vmax));
+        for (int e = 0; e < 4; e++) f[e] = E::to(x[e]);
+      };
+      float lam[OPEN];  // exponent of a token's values: the same part as a block's scale
+      bool there[OPEN];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          float dot = 0.0f;  // of row r, over the thread's dims
+      for (int y = 0; y < OPEN; y++) {
+        there[y] = y < n_open && !(hide && hide[closed + warp + y * kQsWarps]);
+        float vmax = 0.0f;
+        if (there[y]) {
 #pragma unroll
-          for (int k = 0; k < S::KS; k++) {
-            const int d0 = HDP >= 64 ? (k / 4 * 4 + cq) * 16 + k % 4 * 4 : cq * 8 + k * 4;
-            float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int x = QT - 1; x >= 0; x--) {
-              const uint2 bf = qf[((k * NT + n) * QT + x) * 32 + lane];
-              const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&bf.x));
-              const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&bf.y));
-              q[0] += lo.x;
-              q[1] += lo.y;
-              q[2] += hi.x;
-              q[3] += hi.y;
+          for (int d = 0; d < HDP / 8; d += 4)
+            if (EXACT || r * (HDP / 8) + d < hd) {
+              float f4[4];
+              quad(f4, vb + y * hd + d);
+              vmax = fmaxf(vmax, fmaxf(fmaxf(fabsf(f4[0]), fabsf(f4[1])), fmaxf(fabsf(f4[2]), fabsf(f4[3]))));
             }
-            if (d0 < hd) {
+        }
+        lam[y] = vmax;
+      }
 #pragma unroll
-              for (int e = 0; e < 4; e++) dot = fmaf(q[e], E::to(kr[d0 + e]), dot);
-            }
+      for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+        for (int y = 0; y < OPEN; y++) lam[y] = fmaxf(lam[y], __shfl_xor_sync(0xffffffffu, lam[y], d));
+#pragma unroll
+      for (int y = 0; y < OPEN; y++) lam[y] = scale_exponent(lam[y]);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float dot[OPEN];  // of row r, over the thread's dims
+#pragma unroll
+        for (int y = 0; y < OPEN; y++) dot[y] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < S::KS; k++) {
+          const int d0 = HDP >= 64 ? (k / 4 * 4 + cq) * 16 + k % 4 * 4 : cq * 8 + k * 4;
+          float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int x = QT - 1; x >= 0; x--) {
+            const uint2 bf = qf[((k * NT + n) * QT + x) * 32 + lane];
+            const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&bf.x));
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&bf.y));
+            q[0] += lo.x;
+            q[1] += lo.y;
+            q[2] += hi.x;
+            q[3] += hi.y;
           }
-          dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-          dot += __shfl_xor_sync(0xffffffffu, dot, 2);
-          dot *= fac[n * 8 + r];
-          float w[2], al[2];
-          bool on[2];
+          if (EXACT || d0 < hd) {
+#pragma unroll
+            for (int y = 0; y < OPEN; y++)
+              if (there[y]) {
+                float f4[4];
+                quad(f4, kb + y * hd + d0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) dot[y] = fmaf(q[e], f4[e], dot[y]);
+              }
+          }
+        }
+        float w[OPEN][2], al[2];
+#pragma unroll
+        for (int y = 0; y < OPEN; y++) {
+          dot[y] += __shfl_xor_sync(0xffffffffu, dot[y], 1);
+          dot[y] += __shfl_xor_sync(0xffffffffu, dot[y], 2);
+          dot[y] *= fac[n * 8 + r];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const float x = __shfl_sync(0xffffffffu, dot, (2 * cq + e) * 4);
-            on[e] = t < seen[n][e];
-            const float mn = on[e] ? fmaxf(m[n][e], x + lam) : m[n][e];
-            const float ref = mn == -INFINITY ? 0.0f : mn;
-            al[e] = ex2(m[n][e] - ref);
-            w[e] = on[e] ? ex2(x - ref) : 0.0f;
-            m[n][e] = mn;
-            l[n][e] = l[n][e] * al[e] + (r == 0 ? w[e] : 0.0f);
-            w[e] *= 16384.0f;
+            const float x = __shfl_sync(0xffffffffu, dot[y], (2 * cq + e) * 4);
+            w[y][e] = there[y] && closed + warp + y * kQsWarps < seen[n][e] ? x : -INFINITY;
           }
+        }
 #pragma unroll
-          for (int j = 0; j < MT; j++)
+        for (int e = 0; e < 2; e++) {
+          float mn = m[n][e];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const int d = 2 * j + (e >> 1);
-              const float v = r * (HDP / 8) + d < hd ? E::to(vr[d]) : 0.0f;
-              const float y = o[j][n][e] * al[e & 1];
-              o[j][n][e] = on[e & 1] ? fmaf(w[e & 1], v, y) : y;
+          for (int y = 0; y < OPEN; y++) mn = fmaxf(mn, w[y][e] + lam[y]);
+          const float ref = mn == -INFINITY ? 0.0f : mn;
+          al[e] = ex2(m[n][e] - ref);
+          m[n][e] = mn;
+          l[n][e] *= al[e];
+#pragma unroll
+          for (int y = 0; y < OPEN; y++) {
+            w[y][e] = ex2(w[y][e] - ref);
+            if (r == 0) l[n][e] += w[y][e];
+            w[y][e] *= 16384.0f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[j][n][e] *= al[e & 1];
+#pragma unroll
+        for (int y = 0; y < OPEN; y++) {
+          if (!there[y]) continue;
+          // a weight of 0 may stand for a position that the row does not see: its values are left out
+          const bool on0 = w[y][0] != 0.0f, on1 = w[y][1] != 0.0f;
+#pragma unroll
+          for (int d = 0; d < HDP / 8; d += 4)
+            if (EXACT || r * (HDP / 8) + d < hd) {
+              float f4[4];
+              quad(f4, vb + y * hd + d);
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const int j = (d + e) / 2, z = e % 2 * 2;
+                if (on0) o[j][n][z] = fmaf(w[y][0], f4[e], o[j][n][z]);
+                if (on1) o[j][n][z + 1] = fmaf(w[y][1], f4[e], o[j][n][z + 1]);
+              }
             }
         }
       }
@@ -851,7 +912,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
           for (int e = 0; e < 4; e++) O[e] = res[row * S::ORow + d + e];
         }
-        const int token = s.row0 + (x0 + row) / G, head = kvh * G + (x0 + row) % G;
+        const int tok = token_of(x0 + row), token = s.row0 + tok, head = kvh * G + x0 + row - tok * G;
         if (splits > kQsCluster) {  // merged with the other clusters' by k_q8_merge
           float* y = a.ws + (((size_t)token * a.heads + head) * groups + group) * (hd + 4);
           *reinterpret_cast<float4*>(y + d) = make_float4(O[0], O[1], O[2], O[3]);
@@ -1050,6 +1111,8 @@ void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& args, cudaStre
   Q8Attend a = args;
   a.out_aligned = aligned16(a.out.p, a.out.token, a.out.head, 0, esize_of(c.type));
   a.q_aligned = aligned16(a.q.p, a.q.token, a.q.head, 0, esize_of(c.type));
+  a.group = a.heads / c.kvh;
+  a.group_inv = (unsigned)(0xFFFFFFFFull / (unsigned)a.group + 1);
   a.tiled = q8_tiles(c, b, a);
   if (a.tiled) {
     q8_attend_tiles(c, b, a, st);

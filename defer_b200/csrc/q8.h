@@ -79,6 +79,8 @@ struct Q8Attend {
   // set by q8_attend
   int q_aligned, out_aligned;  // the rows start on 16 bytes
   int tiled;                   // sequences of more than kQ8FewRows rows are q8_attend_tiles'
+  int group;                   // heads of a key head
+  unsigned group_inv;          // 2^32 / group, rounded up
 };
 // Rows of a sequence and key head up to which the streaming kernel takes them
 // all: 4 passes over the cache with 16 rows each.
