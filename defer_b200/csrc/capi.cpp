@@ -48,6 +48,7 @@ int guard(F&& f) {
     f();
     return defer::kOk;
   } catch (const defer::Error& e) {
+    if (e.status == defer::kCuda) cudaGetLastError();  // reported here: not again by a later call's check
     defer::set_last_error(e.what());
     return e.status;
   } catch (const std::bad_alloc&) {
@@ -767,6 +768,7 @@ int defer_q8_attend(const defer_q8_cache* cache, const defer_q8_batch* batch, co
     q8_heads(c, heads);
     q8_check(std::isfinite(scale), "scale must be finite");
     q8_check(!masked || mask_stride == 0 || mask_stride >= c.cap, "masked must have a byte for each of cap positions");
+    q8_check((uint64_t)b.tokens * heads <= 1u << 30, "tokens * heads must be at most 2^30");
     if (b.n == 0 || b.tokens == 0) return;
     need(lens, "lens");
     need(q, "q");

@@ -70,7 +70,10 @@ __device__ __forceinline__ bool unit_of(int n, int heads2, int per_seq, int& blk
 }
 
 // ------------------------------------------------------------------ append
-// One warp per (sequence, head, K or V, block). It holds the block in
+// Bound by latency when a call brings a token a sequence (512 of them: 8.5 us
+// with cold caches), else by the instructions of the codes: 8 prompts of 666
+// to 1999 tokens (8B heads, bf16 to e4m3) take 33 us, of which the bytes would
+// be 5. One warp per (sequence, head, K or V, block). It holds the block in
 // registers: 16 bytes of input a lane and step, so a step reads 512
 // contiguous bytes, then the block's largest value by shuffles, then the
 // codes. The warp of a sequence's first block also stores the open block
@@ -171,8 +174,10 @@ __global__ void __launch_bounds__(128, HDMAX <= 64 ? 10 : HDMAX <= 128 ? 7 : 4) 
 }
 
 // -------------------------------------------------------------------- read
-// One warp per (sequence, head, K or V, block); 16 bytes of output a lane
-// and step, stored past L1.
+// Bound by the bytes: 8 sessions of 3001 to 4096 positions (8B heads, e4m3 to
+// bf16) in 32 us, 5.4 TB/s. One warp per (sequence, head, K or V, block); 16
+// bytes of output a lane and step, the block's loads sent off together, loads
+// and stores past L1.
 template <int TYPE, int KIND, int HD>
 __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __restrict__ lens,
                                                  const int* __restrict__ start, const int* __restrict__ slots,
@@ -269,16 +274,26 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // distributed shared memory, and up to 8 splits need no workspace and no
 // second launch. The clusters of longer sequences leave theirs in the
 // workspace, for k_q8_merge. The number of splits follows from the sequence's
-// length alone, so its result does not depend on the batch it runs in. A warp loads its steps
-// (4 KB of K and V) straight into the registers of the matrix instruction:
-// the order of the dims inside the score product, and of the dims of the
-// output, is free, so a thread takes 16 neighbouring bytes of a position
-// wherever it can, and nothing of the stream passes through shared memory.
-// K is loaded again as soon as its scores are done and V as soon as its
-// products are, and every lane asks for one 128-byte line of a step further
-// on to be brought into L2, which keeps enough bytes on their way. The open
-// block (fp32 or 16-bit tokens) is added at the end by the last split, a
-// token a warp, in fp32.
+// length and rows alone, so its result does not depend on the batch it runs
+// in. A warp loads its steps (4 KB of K and V) straight into the registers of
+// the matrix instruction: the order of the dims inside the score product, and
+// of the dims of the output, is free, so a thread takes 16 neighbouring bytes
+// of a position wherever it can, and nothing of the stream passes through
+// shared memory. K is loaded again as soon as its scores are done and V as soon
+// as its products are, and every lane asks for one 128-byte line of a step
+// further on to be brought into L2, which keeps enough bytes on their way. The
+// open block (fp32 or 16-bit tokens) is added at the end by the last split, in
+// fp32.
+//
+// What bounds it: the issue of instructions, not the bytes. A step of 16
+// positions and 128 dims costs a warp about 370 instructions (112 of them turn
+// codes into fp16), a CTA's start, merges and open block about 5 us beside its
+// steps of 0.9 us. 8 sessions of 4096 positions (8B heads, fp32): 27 us, 2.5
+// TB/s; one sequence of 131077 (bf16): 62 us, 4.3 TB/s; 512 sessions of 16 to
+// 767 (135M heads): 37 us, 2.3 TB/s. CTAs of 4 warps let 4 of them overlap on
+// an SM: with 8 warps the last one took 43 us, 127 short sequences 78 instead
+// of 49. A ring of asynchronous copies in shared memory in place of the direct
+// loads: 53 us.
 constexpr int kQsWarps = 4;
 constexpr int kQsCluster = 8;     // splits of a cluster
 constexpr int kQsMaxSplits = 64;  // of a sequence
@@ -302,15 +317,18 @@ constexpr size_t qs_smem() {
 }
 
 // Splits of a sequence of `rows` rows a key head with `closed` positions in
-// closed blocks. Up to 16 rows: of 4 units or more up to 8 splits (a single
-// short sequence is a matter of latency: 14 us instead of 16 for 1041 positions
-// of the 135M heads), of 8 units or more beyond (a CTA's start and its merges
-// cost about 5 steps). More rows are many CTAs anyway: of 8 units or more (512
-// rows over 2048 positions of the 135M heads: 43 us instead of 65).
+// closed blocks. Up to 16 rows: of 4 units or more (a single short sequence is
+// a matter of latency: 14 us instead of 16 for 1041 positions of the 135M
+// heads), up to the 8 that one cluster merges; of 16 units or more when that
+// makes more of them (a CTA's start and its merges cost about 5 units: 64
+// sequences of up to 8191 positions take 150 us, 175 with 8 units). More rows
+// are many CTAs anyway: of 8 units or more (512 rows over 2048 positions of the
+// 135M heads: 43 us instead of 65).
 template <int HDP>
 __host__ __device__ __forceinline__ int qs_splits(int closed, int64_t rows) {
   const int units = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT;
-  const int n = rows > 16 || units >= 64 ? units / 8 : units / 4 < kQsCluster ? units / 4 : kQsCluster;
+  const int least = rows > 16 ? 8 : 4;
+  const int n = units >= 16 * kQsCluster ? units / 16 : units / least < kQsCluster ? units / least : kQsCluster;
   return n < 1 ? 1 : n > kQsMaxSplits ? kQsMaxSplits : n;
 }
 
@@ -646,6 +664,11 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
       float lam[S::NG];
 #pragma unroll
       for (int g = 0; g < S::NG; g++) lam[g] = scale_exponent(vs[g]);
+      float rvs[S::NG];
+      if constexpr (TYPE == kQ8F16) {
+#pragma unroll
+        for (int g = 0; g < S::NG; g++) rvs[g] = __fdiv_rn(1.0f, vs[g] * 16384.0f);
+      }
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         float ref[2], al[2];
@@ -674,11 +697,21 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {  // rows r, then r + 8
             float p0 = ex2(sc[g][n][e] - ref[0]), p1 = ex2(sc[g][n][e + 1] - ref[1]);
-            l[n][0] += p0;
-            l[n][1] += p1;
+            float s0 = p0, s1 = p1;  // what the sums take
             p0 = p0 * vs[g] * 16384.0f;  // in this order: the scale of hidden positions may be near the largest number
             p1 = p1 * vs[g] * 16384.0f;
             const __half2 hi = __floats2half2_rn(p0, p1);
+            if constexpr (TYPE == kQ8F16) {
+              // an fp16 result has the bits of the rounded weights: the sums take those, so that
+              // a weight's rounding cancels where one position has most of the weight
+              if (vs[g] > 0.0f) {
+                const float2 back = __half22float2(hi);
+                s0 = back.x * rvs[g];
+                s1 = back.y * rvs[g];
+              }
+            }
+            l[n][0] += s0;
+            l[n][1] += s1;
             p[g][n][0][e >> 1] = transpose8(h2_bits(hi));
             if constexpr (QT == 2) {
               const float2 back = __half22float2(hi);
@@ -744,7 +777,8 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
             if (EXACT || r * (HDP / 8) + d < hd) {
               float f4[4];
               quad(f4, vb + y * hd + d);
-              vmax = fmaxf(vmax, fmaxf(fmaxf(fabsf(f4[0]), fabsf(f4[1])), fmaxf(fabsf(f4[2]), fabsf(f4[3]))));
+#pragma unroll
+              for (int e = 0; e < 4; e++) vmax = fmaxf(vmax, fabsf(f4[e]) <= FLT_MAX ? fabsf(f4[e]) : 0.0f);
             }
         }
         lam[y] = vmax;
@@ -786,6 +820,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
           }
         }
         float w[OPEN][2], al[2];
+        bool on[OPEN][2];  // the row sees the token
 #pragma unroll
         for (int y = 0; y < OPEN; y++) {
           dot[y] += __shfl_xor_sync(0xffffffffu, dot[y], 1);
@@ -794,7 +829,8 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const float x = __shfl_sync(0xffffffffu, dot[y], (2 * cq + e) * 4);
-            w[y][e] = there[y] && closed + warp + y * kQsWarps < seen[n][e] ? x : -INFINITY;
+            on[y][e] = there[y] && closed + warp + y * kQsWarps < seen[n][e];
+            w[y][e] = on[y][e] ? x : -INFINITY;
           }
         }
 #pragma unroll
@@ -820,8 +856,6 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
         for (int y = 0; y < OPEN; y++) {
           if (!there[y]) continue;
-          // a weight of 0 may stand for a position that the row does not see: its values are left out
-          const bool on0 = w[y][0] != 0.0f, on1 = w[y][1] != 0.0f;
 #pragma unroll
           for (int d = 0; d < HDP / 8; d += 4)
             if (EXACT || r * (HDP / 8) + d < hd) {
@@ -830,8 +864,8 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
               for (int e = 0; e < 4; e++) {
                 const int j = (d + e) / 2, z = e % 2 * 2;
-                if (on0) o[j][n][z] = fmaf(w[y][0], f4[e], o[j][n][z]);
-                if (on1) o[j][n][z + 1] = fmaf(w[y][1], f4[e], o[j][n][z + 1]);
+                if (on[y][0]) o[j][n][z] = fmaf(w[y][0], f4[e], o[j][n][z]);
+                if (on[y][1]) o[j][n][z + 1] = fmaf(w[y][1], f4[e], o[j][n][z + 1]);
               }
             }
         }

@@ -8,9 +8,11 @@ have a device pointer (torch CUDA tensors; torch itself is not imported).
     q8_read(cache, k_out, v_out, lens)      # values back
 
 Every call launches on `stream` (a cudaStream_t as an integer), by default
-torch's current stream of the cache's device, allocates nothing on the device
-and waits for nothing, so it may be captured into a CUDA graph. The arrays
-must stay allocated until the stream has run the call.
+torch's current stream of the cache's device, and waits for nothing, so it may
+be captured into a CUDA graph (make one such call before the capture: CUDA
+loads device code at a kernel's first launch). Nothing is allocated on the
+device but the workspace of long sequences (q8_attend). The arrays must stay
+allocated until the stream has run the call.
 """
 from __future__ import annotations
 
@@ -37,7 +39,10 @@ def _refuse(what: str):
 
 def _stream_of(device: int) -> int:
     t = sys.modules.get("torch")
-    return t._C._cuda_getCurrentRawStream(device) if t is not None else 0
+    if t is None:
+        return 0
+    raw = getattr(t._C, "_cuda_getCurrentRawStream", None)  # a tenth of the public call's time
+    return raw(device) if raw is not None else t.cuda.current_stream(device).cuda_stream
 
 
 _names = {}  # dtype object -> its name (str() of a torch dtype costs more than a call's other checks)
@@ -213,7 +218,7 @@ def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: 
     return out
 
 
-_LONG = 4500  # shorter sequences need no workspace, whatever the head size
+_LONG = 9000  # shorter sequences need no workspace, whatever the head size
 
 
 def _workspace_bytes(cache: Q8Cache, batch: bytes, max_len: int, heads: int) -> int:

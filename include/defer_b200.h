@@ -270,8 +270,11 @@ DEFER_API double defer_log_softmax_at(const float* logits, size_t n, size_t idx)
  * a cache of a quarter of the bytes, for callers whose sessions no longer fit
  * or whose steps are bound by reading the cache. These operators work on the
  * caller's own device buffers (as defer_forward_noalloc does), allocate
- * nothing, synchronise nothing and may be captured into a CUDA graph; calls
- * that write one cache must be ordered by the caller (one stream, events).
+ * nothing, synchronise nothing and may be captured into a CUDA graph (after
+ * one such call outside the capture: CUDA loads device code at a kernel's
+ * first launch). Calls that write one cache must be ordered by the caller
+ * (one stream, events). A bounded wait that runs out in defer_q8_attend fills
+ * the rows with NaN and sets bit 2 of the status word.
  *
  * One layer of the cache, every pointer 16-byte aligned memory of `device`:
  *   codes  [slots][kv_heads][cap][head_dim]   int8 (kind 0) or e4m3 (kind 1)

@@ -230,7 +230,8 @@ LENS = [1, 15, 16, 17, 31, 64, 127, 128, 129, 255, 300, 641]
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
-@pytest.mark.parametrize("heads,kvh,hd", [(9, 3, 64), (4, 1, 128), (2, 2, 16), (8, 1, 256), (20, 2, 80), (32, 32, 32)])
+@pytest.mark.parametrize("heads,kvh,hd", [(9, 3, 64), (4, 1, 128), (2, 2, 16), (8, 1, 256), (20, 2, 80), (32, 32, 32),
+                                          (6, 2, 144), (4, 4, 48)])
 def test_attend_single_rows(dtype, kind, heads, kvh, hd):
     c = Case(len(LENS), kvh, 656, hd, kind, dtype, seed=heads + hd)
     slots = list(range(len(LENS)))
@@ -291,8 +292,9 @@ def test_hidden_places_may_hold_anything(dtype, rows):
     assert torch.isfinite(out).all()
 
 
-def test_large_and_tiny_scores_and_values():
-    c = Case(4, 1, 192, 64, "int8", F32, seed=8)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_large_and_tiny_scores_and_values(dtype):
+    c = Case(4, 1, 192, 64, "int8", dtype, seed=8)
     k, v = c.randn(4 * 180, 1, 64), c.randn(4 * 180, 1, 64)
     k[180:360] *= 40                      # weights of one position alone
     v[180:360] *= 1e30
@@ -310,9 +312,10 @@ def test_large_and_tiny_scores_and_values():
         c.attend_check([0, 1, 2, 3], [rows] * 4, 2, q=q)
 
 
-def test_a_non_finite_query_stays_in_its_row():
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_a_non_finite_query_stays_in_its_row(dtype):
     for rows in (1, 140):
-        c = Case(2, 1, 160, 64, "int8", F32, seed=1)
+        c = Case(2, 1, 160, 64, "int8", dtype, seed=1)
         c.append([0, 1], [150, 150])
         q = c.randn(2 * rows, 4, 64)
         q[0, 1, 3], q[0, 3, 3] = float("nan"), float("inf")
@@ -339,6 +342,37 @@ def test_lengths_out_of_range_and_rows_behind():
     assert torch.isfinite(out[:4]).all() and (out[4:] == 77.0).all()
     D.q8_attend(c.cache, q, out, ints([0, 0, 0]))  # empty sequences
     assert (out == 0).all()
+
+
+def test_visible_values_that_are_no_numbers():
+    """A NaN or an infinity among the open block's values reaches the rows that see it, and only its own dim."""
+    for dtype in (F32, BF16):
+        for rows in (4, 140):
+            c = Case(1, 1, 192, 64, "int8", dtype, seed=2)
+            k, v = c.randn(172, 1, 64), c.randn(172, 1, 64)
+            v[169, 0, 7], v[170, 0, 9] = float("nan"), float("inf")
+            c.append([0], [172], k, v)
+            q = c.randn(rows, 2, 64)
+            out = torch.empty_like(q)
+            D.q8_attend(c.cache, q, out, ints([172]))
+            seen = 172 - (rows - 1) + torch.arange(rows, device="cuda")
+            for dim, t, what in ((7, 169, torch.isnan), (9, 170, torch.isinf)):
+                assert torch.equal(what(out[:, :, dim]), (seen > t)[:, None].expand(rows, 2))
+            keep = [d for d in range(64) if d not in (7, 9)]
+            assert torch.isfinite(out[:, :, keep]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 140])
+def test_empty_sequences_and_bad_ones_among_many_rows(rows):
+    for dtype in (F32, BF16):
+        c = Case(4, 2, 192, 64, "e4m3", dtype, seed=4)
+        c.append([0, 1, 2, 3], [190, 3, 20, 160])
+        q = c.randn(5 * rows, 4, 64)
+        out, status = torch.full_like(q, 77.0), ints([0])
+        D.q8_attend(c.cache, q, out, ints([190, 0, 193, 20, 160]), slots=ints([0, 1, 2, -1, 9]), status=status)
+        out = out.view(5, rows, 4, 64)
+        assert torch.isfinite(out[0]).all() and (out[1] == 0).all() and torch.isnan(out[2]).all()
+        assert (out[3] == 77.0).all() and torch.isnan(out[4]).all() and status.item() == 1
 
 
 @pytest.mark.parametrize("rows", [1, 3, 70, 160])
@@ -447,6 +481,74 @@ def test_streams_and_graphs():
     D.q8_attend(c.cache, q, b, lens, stream=st.cuda_stream)
     st.synchronize()
     assert torch.equal(a, b)
+
+
+def test_two_calls_at_once():
+    """Long sequences on two streams, each with a workspace of its own, and two replayed graphs."""
+    c = Case(2, 2, 12016, 128, "int8", BF16, seed=6)
+    c.append([0, 1], [12000, 9990])
+    q = [c.randn(2, 8, 128) for _ in range(2)]
+    want = [D.q8_attend(c.cache, x, torch.empty_like(x), ints([12000, 9990])).clone() for x in q]
+    torch.cuda.synchronize()
+    lens = ints([12000, 9990])
+    st = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(x) for x in q]
+    graphs = []
+    for x, o, s in zip(q, outs, st):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            D.q8_attend(c.cache, x, o, lens)
+        graphs.append(g)
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, st):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+    for _ in range(5):
+        for x, o, s in zip(q, outs, st):
+            o.zero_()
+            s.wait_stream(torch.cuda.current_stream())
+            D.q8_attend(c.cache, x, o, lens, stream=s.cuda_stream)
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """A slot behind 4 GB of codes, and a position whose codes lie 4 GB into its head."""
+    n = 1 << 24
+    cap, hd = n + 64, 256
+    g = torch.Generator("cuda").manual_seed(0)
+    codes = [torch.empty(2, 1, cap, hd, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.empty(2, 1, cap // 16, device="cuda") for _ in range(2)]
+    tails = [torch.zeros(2, 1, 16, hd, dtype=BF16, device="cuda") for _ in range(2)]
+    cache = D.Q8Cache(*codes, *scales, *tails)
+    k, v = (torch.randn(40, 1, hd, device="cuda", generator=g).to(BF16) for _ in range(2))
+    D.q8_append(cache, k, v, ints([n]), slots=ints([1]))
+    twin = Case(1, 1, 64, hd, "int8", BF16)
+    twin.append([0], [40], k, v)
+    back = [torch.zeros(1, 1, 40, hd, dtype=BF16, device="cuda") for _ in range(2)]
+    D.q8_read(cache, *back, ints([n + 40]), start=ints([n]), slots=ints([1]))
+    for got, want in zip(back, twin.values(0)):
+        assert torch.equal(got[0], torch.tensor(want.astype(np.float32), device="cuda").to(BF16))
+    # the positions before those are hidden: codes and scales of any value, as long as they are numbers
+    for x in codes:
+        x[1, 0, :n] = 1
+    for x in scales:
+        x[1, 0, :n // 16] = 1.0
+    masked = torch.zeros(1, cap, dtype=torch.uint8, device="cuda")
+    masked[0, :n] = 1
+    for rows in (1, 80):
+        q = torch.randn(rows, 2, hd, device="cuda", generator=g).to(BF16)
+        out = torch.empty_like(q)
+        D.q8_attend(cache, q, out, ints([n + 40]), slots=ints([1]), masked=masked, causal=False)
+        want, most = attend64(q.double().cpu().numpy(), *twin.values(0), [40] * rows, None, hd ** -0.5)
+        assert far(out, want) <= tolerance(BF16, most)
 
 
 def test_generation_together():

@@ -61,7 +61,8 @@ def test_null_descriptors_are_refused():
 
 @pytest.mark.parametrize("kw", [dict(b=batch(tokens=3)), dict(b=batch(n=5, tokens=5)), dict(b=batch(n=0)), dict(lens=None),
                                 dict(heads=3), dict(heads=0), dict(q=None), dict(out=None), dict(ot=192), dict(oh=32),
-                                dict(masked=P, ms=63), dict(scale=float("nan")), dict(scale=float("inf"))])
+                                dict(masked=P, ms=63), dict(scale=float("nan")), dict(scale=float("inf")),
+                                dict(b=batch(n=4, tokens=1 << 29), heads=4)])
 def test_attend_refusals(kw):
     assert attend(**kw) == BAD
 
