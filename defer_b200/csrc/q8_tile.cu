@@ -10,7 +10,7 @@
 // rescaled a few times a row instead of at every tile. The tokens of the open
 // block are 16-bit numbers: scaled by a power of two for the block they are
 // fp16 operands like codes (an element 2^30 times smaller than the block's
-// largest loses bits). Output and sums stay in fp32 (tensor memory,
+// largest loses bits). Weights are one fp16 term for bf16 results, two for fp16. Output and sums stay in fp32 (tensor memory,
 // registers).
 //
 // Work: a CTA takes two tiles of 128 rows (rows of the heads that share a key
@@ -54,7 +54,6 @@ constexpr unsigned long long kQtWaitNs = 2000000000ull;
 struct QtScales {
   float ks[kQtN / kQ8Block];    // K scale
   float vs64[kQtN / kQ8Block];  // V scale times 2^6
-  float rvs[kQtN / kQ8Block];   // its reciprocal, 0 for a scale of 0
   float lam[kQtN / kQ8Block];   // exponent of the V scale
   uint32_t show[kQtN / 32];     // bit per position: exists and is not hidden
 };
@@ -218,6 +217,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   using E = Elem<TYPE>;
   using T = typename E::T;
   constexpr int CH = HDT / 8;       // 16-byte chunks of an operand row
+  constexpr int PT = TYPE == kQ8F16 ? 2 : 1;  // terms of the weights: fp16 results have the bits of one
   constexpr uint32_t GROUP = CH * 128;  // bytes of 8 operand rows
   extern __shared__ __align__(1024) unsigned char qt_raw[];
   QtShared<HDT>& S = *reinterpret_cast<QtShared<HDT>*>(qt_raw);
@@ -423,29 +423,34 @@ __global__ void __launch_bounds__(kQtThreads, 1)
           tm_wait(w);
           if (j < 3) tm_ld32(v[(j + 1) & 1], ts + (j + 1) * 32);
           hide32(w, j);
-          uint32_t p[16];
+          uint32_t p[16], p2[PT == 2 ? 16 : 1];
 #pragma unroll
           for (int g = 0; g < 2; g++) {
-            const float cs = scale_of(2 * j + g), vs = sc.vs64[2 * j + g], rvs = sc.rvs[2 * j + g];
+            const float cs = scale_of(2 * j + g), vs = sc.vs64[2 * j + g];
             const uint64_t cs2 = f2(cs, cs), vs2 = f2(vs, vs);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
               float p0, p1;
               f2_get(f2_fma(f2(__uint_as_float(w[g * 16 + e]), __uint_as_float(w[g * 16 + e + 1])), cs2, nref), p0, p1);
-              uint64_t pp = f2(ex2(p0), ex2(p1));
-              f2_get(f2_mul(pp, vs2), p0, p1);
-              const __half2 h = __floats2half2_rn(p0, p1);
-              p[g * 8 + e / 2] = h2_bits(h);
-              if constexpr (TYPE == kQ8F16) {  // the sums take the rounded weights (as in k_q8_attend)
-                if (rvs > 0.0f) {
-                  const float2 back = __half22float2(h);
-                  pp = f2_mul(f2(back.x, back.y), f2(rvs, rvs));
-                }
-              }
+              const uint64_t pp = f2(ex2(p0), ex2(p1));
               l2 = f2_add(l2, pp);
+              f2_get(f2_mul(pp, vs2), p0, p1);
+              const __half2 hi = __floats2half2_rn(p0, p1);
+              p[g * 8 + e / 2] = h2_bits(hi);
+              if constexpr (PT == 2) {
+                const float2 back = __half22float2(hi);
+                p2[g * 8 + e / 2] = h2_bits(__floats2half2_rn(p0 - back.x, p1 - back.y));
+              }
             }
           }
-          tm_st16(ts + j * 16, p);
+          // the weights of 32 positions in the place of their scores: one term packed
+          // to the front, two behind each other
+          if constexpr (PT == 2) {
+            tm_st16(ts + j * 32, p);
+            tm_st16(ts + j * 32 + 16, p2);
+          } else {
+            tm_st16(ts + j * 16, p);
+          }
         }
         {
           float l0, l1;
@@ -634,7 +639,6 @@ __global__ void __launch_bounds__(kQtThreads, 1)
             }
             sc.ks[ct] = ks;
             sc.vs64[ct] = vs * 64.0f;
-            sc.rvs[ct] = vs > 0.0f ? __fdiv_rn(1.0f, vs * 64.0f) : 0.0f;
             sc.lam[ct] = scale_exponent(vs);
           }
           qb_arrive(&S.sc_full[n % kQtSlots]);
@@ -667,7 +671,10 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       const uint32_t va = smem_u32(S.v[blk & 1]);
 #pragma unroll
       for (int k = 0; k < kQtN / 16; k++)
-        qt_mma_ts(tm_o[w], tm_s[w] + k * 8, qt_desc(va + k * 2 * GROUP, GROUP, 128), kQtIdesc<HDT, true>, acc || k > 0);
+#pragma unroll
+        for (int z = 0; z < PT; z++)
+          qt_mma_ts(tm_o[w], tm_s[w] + (PT == 2 ? k / 2 * 32 + k % 2 * 8 + z * 16 : k * 8),
+                    qt_desc(va + k * 2 * GROUP, GROUP, 128), kQtIdesc<HDT, true>, acc || k > 0 || z > 0);
     };
     for (int item = first; item < items && ok; item += tiles) {
       const int x0 = item * per_item, x_end = min(x0 + per_item, R);
