@@ -70,18 +70,17 @@ __device__ __forceinline__ bool unit_of(int n, int heads2, int per_seq, int& blk
 }
 
 // ------------------------------------------------------------------ append
-// Bound by latency when a call brings a token a sequence (512 of them: 8.5 us
-// with cold caches), else by the instructions of the codes: 8 prompts of 666
-// to 1999 tokens (8B heads, bf16 to e4m3) take 33 us, of which the bytes would
-// be 5. One warp per (sequence, head, K or V, block). It holds the block in
-// registers: 16 bytes of input a lane and step, so a step reads 512
-// contiguous bytes, then the block's largest value by shuffles, then the
-// codes. The warp of a sequence's first block also stores the open block
-// (the tail): it is the only one that reads the old tail, and it does so
-// before it writes.
+// Bound by the latency of its loads: 512 tokens, one a sequence, take 8.5 us
+// with cold caches; 8 prompts of 666 to 1999 tokens (8B heads, bf16 to e4m3) 33
+// us, where the bytes alone would take 10. One warp per (sequence, head, K or
+// V, block). It holds the block in registers: 16 bytes of input a lane and
+// step, so a step reads 512 contiguous bytes, then the block's largest value by
+// shuffles, then the codes. The warp of a sequence's first block also stores
+// the open block (the tail): it is the only one that reads the old tail, and it
+// does so before it writes.
 template <int TYPE, int KIND, int HDMAX, bool EXACT>
-__global__ void __launch_bounds__(128, HDMAX <= 64 ? 10 : HDMAX <= 128 ? 7 : 4) k_q8_append(Q8View c, Q8Batch b, const int* __restrict__ pos, Q8Rows rk,
-                                                   Q8Rows rv, int aligned, int per_seq) {
+__global__ void __launch_bounds__(128, HDMAX <= 64 ? 10 : HDMAX <= 128 ? 7 : 4)
+    k_q8_append(Q8View c, Q8Batch b, const int* __restrict__ pos, Q8Rows rk, Q8Rows rv, int aligned, int per_seq) {
   using E = Elem<TYPE>;
   using T = typename E::T;
   constexpr int VEC = 16 / (int)sizeof(T);             // elements of one step and lane
@@ -249,8 +248,9 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 }
 
 // ------------------------------------------------------------------ attend
-// Attention of a few rows (q8_few_rows) of a sequence and key head: the cache
-// is read once, and everything else is arranged around that stream.
+// Attention of a few rows of a sequence and key head (all of them where the
+// tiles of q8_tile.cu do not serve): 8 or 16 rows read the cache once, and
+// everything else is arranged around that stream.
 //
 // Mathematics. A code is a whole number (or an e4m3 number): exact in fp16,
 // so the scores of a block are (codes . q) * s_K and its share of the output
