@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // with them, P' = 2^(x + log2 s_V - m) with the running maximum m taken over
 // x + floor(log2 s_V) (x: score in base 2): times 2^14 they use fp16's whole
 // range, relative to the largest contribution to the output whatever the
-// scales of the other blocks are: one term for bf16 results; two for fp32, and
-// for fp16, whose own 11 bits one term would double the error of. The sum of the
+// scales of the other blocks are, in two terms (22 bits; with one, 11 bits, the
+// errors of 16-bit results are more than their own rounding). The sum of the
 // weights themselves, 2^(x - m), stays in fp32. fp32 caches add the products
 // of each step to fp32 registers (a long chain of sums inside the tensor core
 // would lose bits that a 16-bit result does not have). Softmax: running
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
   using S = QsShape<HDP>;
   using E = Elem<TYPE>;
   using T = typename E::T;
-  constexpr int QT = TYPE == kQ8F32 ? 2 : 1, PT = TYPE == kQ8Bf16 ? 1 : 2;  // terms of q and of the weights
+  constexpr int QT = TYPE == kQ8F32 ? 2 : 1;  // terms of q; the weights have two
   constexpr int ROWS = 8 * NT, MT = HDP / 16;
   constexpr int WO = ROWS * S::ORow;  // floats of a warp's result; before that, its tokens of the open block
   constexpr int KL = S::KW < 4 ? S::KW : 4, VL = S::VW < 4 ? S::VW : 4;  // words of one load
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
           }
       }
       // ---- running maximum of weight times value scale, weights, their sum
-      uint32_t p[S::NG][NT][PT][2];
+      uint32_t p[S::NG][NT][2][2];
       float lam[S::NG];
 #pragma unroll
       for (int g = 0; g < S::NG; g++) lam[g] = scale_exponent(vs[g]);
@@ -700,10 +700,8 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
             p1 = p1 * vs[g] * 16384.0f;
             const __half2 hi = __floats2half2_rn(p0, p1);
             p[g][n][0][e >> 1] = transpose8(h2_bits(hi));
-            if constexpr (PT == 2) {
-              const float2 back = __half22float2(hi);
-              p[g][n][1][e >> 1] = transpose8(h2_bits(__floats2half2_rn(p0 - back.x, p1 - back.y)));
-            }
+            const float2 back = __half22float2(hi);
+            p[g][n][1][e >> 1] = transpose8(h2_bits(__floats2half2_rn(p0 - back.x, p1 - back.y)));
           }
       }
       // ---- values
@@ -724,7 +722,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
             for (int n = 0; n < NT; n++) {
               if constexpr (TYPE != kQ8F32) {
 #pragma unroll
-                for (int q = 0; q < PT; q++) mma16816(o[j][n], af, p[g][n][q][0], p[g][n][q][1]);
+                for (int q = 0; q < 2; q++) mma16816(o[j][n], af, p[g][n][q][0], p[g][n][q][1]);
               } else {
                 float d[4];
                 mma16816_zero(d, af, p[g][n][0][0], p[g][n][0][1]);

@@ -10,8 +10,8 @@
 // rescaled a few times a row instead of at every tile. The tokens of the open
 // block are 16-bit numbers: scaled by a power of two for the block they are
 // fp16 operands like codes (an element 2^30 times smaller than the block's
-// largest loses bits). Weights are one fp16 term for bf16 results, two for fp16. Output and sums stay in fp32 (tensor memory,
-// registers).
+// largest loses bits). Weights are two fp16 terms (22 bits). Output and sums stay
+// in fp32 (tensor memory, registers).
 //
 // Work: a CTA takes two tiles of 128 rows (rows of the heads that share a key
 // head, token after token), so that a converted block of 128 positions feeds
@@ -156,9 +156,19 @@ __device__ __forceinline__ void tm_ld32(uint32_t (&v)[32], uint32_t a) {
       : "r"(a)
       : "memory");
 }
+__device__ __forceinline__ void tm_ld16(uint32_t (&v)[16], uint32_t a) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : QT_R8(v, 0), QT_R8(v, 8)
+      : "r"(a)
+      : "memory");
+}
 #define QT_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
 __device__ __forceinline__ void tm_wait(uint32_t (&v)[32]) {  // every load of the thread; v is used only behind it
   asm volatile("tcgen05.wait::ld.sync.aligned;" : QT_RW8(v, 0), QT_RW8(v, 8), QT_RW8(v, 16), QT_RW8(v, 24) : : "memory");
+}
+__device__ __forceinline__ void tm_wait(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : QT_RW8(v, 0), QT_RW8(v, 8) : : "memory");
 }
 __device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t (&v)[32]) {
   asm volatile(
@@ -217,7 +227,6 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   using E = Elem<TYPE>;
   using T = typename E::T;
   constexpr int CH = HDT / 8;       // 16-byte chunks of an operand row
-  constexpr int PT = TYPE == kQ8F16 ? 2 : 1;  // terms of the weights: fp16 results have the bits of one
   constexpr uint32_t GROUP = CH * 128;  // bytes of 8 operand rows
   extern __shared__ __align__(1024) unsigned char qt_raw[];
   QtShared<HDT>& S = *reinterpret_cast<QtShared<HDT>*>(qt_raw);
@@ -352,45 +361,38 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         qt_after();
-        // positions of the block that the row sees, 32 to a word
-        uint32_t show[4];
-        bool all = true;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
+        // positions j * 32 .. + 31 of the block that the row sees
+        auto shown = [&](int j) {
           const int n = seen - t * kQtN - j * 32;
-          show[j] = sc.show[j] & (n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u);
-          all &= show[j] == 0xffffffffu;
-        }
-        all = __all_sync(0xffffffffu, all);
-        // A row's scores of 32 positions from tensor memory; hidden ones are -inf.
-        auto hide32 = [&](uint32_t (&v)[32], int j) {
+          return sc.show[j] & (n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u);
+        };
+        const bool all = __all_sync(0xffffffffu, (shown(0) & shown(1) & shown(2) & shown(3)) == 0xffffffffu);
+        // A row's scores from tensor memory, from position `at` of the block on; hidden ones are -inf.
+        auto cover = [&](auto& v, int at) {
           if (all) return;
+          const uint32_t w = shown(at >> 5) >> (at & 31);
 #pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (!(show[j] >> e & 1)) v[e] = 0xff800000u;
+          for (int e = 0; e < (int)(sizeof(v) / sizeof(v[0])); e++)
+            if (!(w >> e & 1)) v[e] = 0xff800000u;
         };
         // Scale of a block's scores: never 0, which would turn -inf into NaN;
         // scores (below 2^30) times this least one are 0 to every bit that counts.
         auto scale_of = [&](int g) { return fmaxf(sc.ks[g] * fs, 1.0e-36f); };
-        uint32_t v[2][32];  // one part is worked on while the next one comes
+        uint32_t z[2][16];  // one part is worked on while the next one comes
         // ---- the largest score with its value scale
         float mx = -INFINITY;
-        tm_ld32(v[0], ts);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          uint32_t(&w)[32] = v[j & 1];
+        tm_ld16(z[0], ts);
+#pragma unroll 2
+        for (int g = 0; g < kQtN / 16; g++) {
+          uint32_t(&w)[16] = z[g & 1];
           tm_wait(w);
-          if (j < 3) tm_ld32(v[(j + 1) & 1], ts + (j + 1) * 32);
-          else tm_ld32(v[0], ts);  // the second pass begins
-          hide32(w, j);
+          tm_ld16(z[(g + 1) & 1], g + 1 < kQtN / 16 ? ts + (g + 1) * 16 : ts);  // the last one: for the second pass
+          cover(w, g * 16);
+          float y = __uint_as_float(w[0]);
 #pragma unroll
-          for (int g = 0; g < 2; g++) {
-            float y = __uint_as_float(w[g * 16]);
-#pragma unroll
-            for (int e = 1; e < 15; e += 2) y = max3(y, __uint_as_float(w[g * 16 + e]), __uint_as_float(w[g * 16 + e + 1]));
-            y = fmaxf(y, __uint_as_float(w[g * 16 + 15]));
-            mx = fmaxf(mx, fmaf(y, scale_of(2 * j + g), sc.lam[2 * j + g]));
-          }
+          for (int e = 1; e < 15; e += 2) y = max3(y, __uint_as_float(w[e]), __uint_as_float(w[e + 1]));
+          y = fmaxf(y, __uint_as_float(w[15]));
+          mx = fmaxf(mx, fmaf(y, scale_of(g), sc.lam[g]));
         }
         // ---- move the reference when it has fallen far behind
         if (t == 0) {
@@ -417,40 +419,28 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         // ---- weights over the scores
         const uint64_t nref = f2(-ref, -ref);
         uint64_t l2 = f2(0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          uint32_t(&w)[32] = v[j & 1];
+#pragma unroll 2
+        for (int g = 0; g < kQtN / 16; g++) {
+          uint32_t(&w)[16] = z[g & 1];
           tm_wait(w);
-          if (j < 3) tm_ld32(v[(j + 1) & 1], ts + (j + 1) * 32);
-          hide32(w, j);
-          uint32_t p[16], p2[PT == 2 ? 16 : 1];
+          if (g + 1 < kQtN / 16) tm_ld16(z[(g + 1) & 1], ts + (g + 1) * 16);
+          cover(w, g * 16);
+          const float cs = scale_of(g), vs = sc.vs64[g];
+          const uint64_t cs2 = f2(cs, cs), vs2 = f2(vs, vs);
+          uint32_t p[16];  // the weights of 16 positions: 8 words of the first terms, 8 of the second ones
 #pragma unroll
-          for (int g = 0; g < 2; g++) {
-            const float cs = scale_of(2 * j + g), vs = sc.vs64[2 * j + g];
-            const uint64_t cs2 = f2(cs, cs), vs2 = f2(vs, vs);
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float p0, p1;
-              f2_get(f2_fma(f2(__uint_as_float(w[g * 16 + e]), __uint_as_float(w[g * 16 + e + 1])), cs2, nref), p0, p1);
-              const uint64_t pp = f2(ex2(p0), ex2(p1));
-              l2 = f2_add(l2, pp);
-              f2_get(f2_mul(pp, vs2), p0, p1);
-              const __half2 hi = __floats2half2_rn(p0, p1);
-              p[g * 8 + e / 2] = h2_bits(hi);
-              if constexpr (PT == 2) {
-                const float2 back = __half22float2(hi);
-                p2[g * 8 + e / 2] = h2_bits(__floats2half2_rn(p0 - back.x, p1 - back.y));
-              }
-            }
+          for (int e = 0; e < 16; e += 2) {
+            float p0, p1;
+            f2_get(f2_fma(f2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])), cs2, nref), p0, p1);
+            const uint64_t pp = f2(ex2(p0), ex2(p1));
+            l2 = f2_add(l2, pp);
+            f2_get(f2_mul(pp, vs2), p0, p1);
+            const __half2 hi = __floats2half2_rn(p0, p1);
+            p[e / 2] = h2_bits(hi);
+            const float2 back = __half22float2(hi);
+            p[8 + e / 2] = h2_bits(__floats2half2_rn(p0 - back.x, p1 - back.y));
           }
-          // the weights of 32 positions in the place of their scores: one term packed
-          // to the front, two behind each other
-          if constexpr (PT == 2) {
-            tm_st16(ts + j * 32, p);
-            tm_st16(ts + j * 32 + 16, p2);
-          } else {
-            tm_st16(ts + j * 16, p);
-          }
+          tm_st16(ts + g * 16, p);  // in the place of their scores
         }
         {
           float l0, l1;
@@ -672,8 +662,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
 #pragma unroll
       for (int k = 0; k < kQtN / 16; k++)
 #pragma unroll
-        for (int z = 0; z < PT; z++)
-          qt_mma_ts(tm_o[w], tm_s[w] + (PT == 2 ? k / 2 * 32 + k % 2 * 8 + z * 16 : k * 8),
+        for (int z = 0; z < 2; z++)
+          qt_mma_ts(tm_o[w], tm_s[w] + k * 16 + z * 8,
                     qt_desc(va + k * 2 * GROUP, GROUP, 128), kQtIdesc<HDT, true>, acc || k > 0 || z > 0);
     };
     for (int item = first; item < items && ok; item += tiles) {
