@@ -310,43 +310,47 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       // of input a lane): times 2^up a row's largest element is in [2^14, 2^15).
       constexpr int RL = CH;             // lanes of a row
       constexpr int RI = 32 / RL;        // rows of a load
+      // A tile that sees nothing has no products: no operands, and no arrival that
+      // the issuing thread does not wait for (two in a row would pass it by).
+      if (nb) {
 #pragma unroll 4
-      for (int r0 = 0; r0 < 32; r0 += RI) {
-        const int rr = (warp & 3) * 32 + r0 + lane / RL, ch = lane % RL, y = xt + rr;
-        const bool there = y < x_end && ch * 8 < hd;
-        const T* q = static_cast<const T*>(a.q.p) + (int64_t)(s.row0 + (there ? y : 0) / G) * a.q.token +
-                     (int64_t)(kvh * G + (there ? y : 0) % G) * a.q.head + (there ? ch * 8 : 0);
-        __align__(16) T z[8];
-        if (a.q_aligned) {
-          *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>(q);
-        } else {
+        for (int r0 = 0; r0 < 32; r0 += RI) {
+          const int rr = (warp & 3) * 32 + r0 + lane / RL, ch = lane % RL, y = xt + rr;
+          const bool there = y < x_end && ch * 8 < hd;
+          const T* q = static_cast<const T*>(a.q.p) + (int64_t)(s.row0 + (there ? y : 0) / G) * a.q.token +
+                       (int64_t)(kvh * G + (there ? y : 0) % G) * a.q.head + (there ? ch * 8 : 0);
+          __align__(16) T z[8];
+          if (a.q_aligned) {
+            *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>(q);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 8; e++) z[e] = q[e];
+            for (int e = 0; e < 8; e++) z[e] = q[e];
+          }
+          float v[8], mx = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            v[e] = there ? E::to(z[e]) : 0.0f;
+            mx = fmaxf(mx, fabsf(v[e]));
+          }
+#pragma unroll
+          for (int d = RL / 2; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const int up = mx > 0.0f && mx <= FLT_MAX ? 14 - exponent_of(mx) : 0;
+          const float up0 = exp2i(up / 2), up1 = exp2i(up - up / 2);
+          // the sign of the scale goes into q: a block's largest score is then its largest product
+          const float f = a.scale * 1.4426950408889634f * exp2i(-(up / 2)) * exp2i(up / 2 - up);
+          const float u0 = f < 0.0f ? -up0 : up0;
+          if (ch == 0) S.fac[wg * kQtM + rr] = fabsf(f);
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[e] = h2_bits(__floats2half2_rn(v[2 * e] * u0 * up1, v[2 * e + 1] * u0 * up1));
+          *reinterpret_cast<uint4*>(S.q[wg] + (rr >> 3) * GROUP + (rr & 7) * 16 + ch * 128) =
+              make_uint4(w[0], w[1], w[2], w[3]);
         }
-        float v[8], mx = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          v[e] = there ? E::to(z[e]) : 0.0f;
-          mx = fmaxf(mx, fabsf(v[e]));
-        }
-#pragma unroll
-        for (int d = RL / 2; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        const int up = mx > 0.0f && mx <= FLT_MAX ? 14 - exponent_of(mx) : 0;
-        const float up0 = exp2i(up / 2), up1 = exp2i(up - up / 2);
-        // the sign of the scale goes into q: a block's largest score is then its largest product
-        const float f = a.scale * 1.4426950408889634f * exp2i(-(up / 2)) * exp2i(up / 2 - up);
-        const float u0 = f < 0.0f ? -up0 : up0;
-        if (ch == 0) S.fac[wg * kQtM + rr] = fabsf(f);
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = h2_bits(__floats2half2_rn(v[2 * e] * u0 * up1, v[2 * e + 1] * u0 * up1));
-        *reinterpret_cast<uint4*>(S.q[wg] + (rr >> 3) * GROUP + (rr & 7) * 16 + ch * 128) =
-            make_uint4(w[0], w[1], w[2], w[3]);
+        __syncwarp();
+        qt_proxy();
+        qb_arrive(&S.q_full[wg]);
       }
-      __syncwarp();
       const float fs = S.fac[wg * kQtM + row];
-      qt_proxy();
-      qb_arrive(&S.q_full[wg]);
 
       const uint32_t ts = tm_s[wg] + ((uint32_t)((warp & 3) * 32) << 16);
       const uint32_t to = tm_o[wg] + ((uint32_t)((warp & 3) * 32) << 16);
@@ -671,7 +675,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       const int nb[2] = {blocks_to(min(x0 + kQtM, x_end) - 1), x0 + kQtM < x_end ? blocks_to(x_end - 1) : 0};
       const int all = max(nb[0], nb[1]);
       for (int w = 0; w < 2 && ok; w++)
-        if (x0 + w * kQtM < x_end) ok = qb_wait(&S.q_full[w], n_q[w]++ & 1, failed);
+        if (nb[w]) ok = qb_wait(&S.q_full[w], n_q[w]++ & 1, failed);
       if (!ok) break;
       qt_after();
       if (all) {

@@ -27,7 +27,7 @@ def steps(c, slot):
     return np.concatenate([s, np.repeat(a[:, None] * 2.0 ** -15, len(x), 1)], 1)
 
 
-def check(c, slots, rows, heads, q=None, hidden=None, scale=None, causal=True):
+def check(c, slots, rows, heads, q=None, hidden=None, scale=None, causal=True, **kw):
     """Attention of `rows` random rows of each slot; returns the output."""
     q = c.randn(len(slots) * rows, heads, c.hd) if q is None else q
     out = torch.full_like(q, 77.0)
@@ -37,7 +37,8 @@ def check(c, slots, rows, heads, q=None, hidden=None, scale=None, causal=True):
         masked = torch.zeros(len(slots), c.cap, dtype=torch.uint8, device="cuda")
         for i, h in enumerate(hidden):
             masked[i, :len(h)] = torch.tensor(h, dtype=torch.uint8, device="cuda")
-    D.q8_attend(c.cache, q, out, ints(lens), slots=ints(slots), masked=masked, scale=scale, causal=causal)
+    D.q8_attend(c.cache, q, out, ints(lens), slots=ints(slots), masked=masked, scale=scale, causal=causal,
+                **kw)
     sc = c.hd ** -0.5 if scale is None else scale
     for i, s in enumerate(slots):
         k, v = c.values(s)
