@@ -258,16 +258,18 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // tensor cores (mma m16n8k16, fp32 sums). The other operand is made as exact
 // as the cache's type asks: a q row is scaled by a power of two so that its
 // largest element is in [2^14, 2^15) and held as one fp16 term (bf16 and fp16
-// rows: no bit lost) or two (fp32: 22 bits). The weights take the value scale
-// with them, P' = 2^(x + log2 s_V - m) with the running maximum m taken over
-// x + floor(log2 s_V) (x: score in base 2): times 2^14 they use fp16's whole
-// range, relative to the largest contribution to the output whatever the
-// scales of the other blocks are, in two terms (22 bits; with one, 11 bits, the
-// errors of 16-bit results are more than their own rounding). The sum of the
-// weights themselves, 2^(x - m), stays in fp32. fp32 caches add the products
-// of each step to fp32 registers (a long chain of sums inside the tensor core
-// would lose bits that a 16-bit result does not have). Softmax: running
-// maximum and sum per warp; warps, then splits, are merged in order.
+// rows: no bit lost) or two (fp32: 22 bits). The weights of a block are taken
+// relative to the block's own largest score, P = 2^(x - max_block x) (x: score
+// in base 2), times 2^14 in two fp16 terms: 22 bits, with one term (11 bits)
+// the errors of 16-bit results are more than their own rounding. The block's
+// products P . codes come out of the tensor core by themselves and are added to
+// fp32 registers times 2^(max_block x - m) s_V, m the running maximum of the
+// scores: no block's values, however large, cost the others bits, and nothing
+// is summed in a long chain inside the tensor core. The sum of the weights is
+// relative to m too. Softmax: running maximum and sum per warp; warps, then
+// splits, are merged in order. Values near fp32's largest number would make the
+// sum of weights times values infinite where their quotient is not: scales from
+// 2^73 on raise a power of two that the warp's output is held in units of.
 //
 // Work. The positions of the closed blocks are cut into units of 4 warp
 // steps, the units into splits, one CTA each, 8 splits of a (sequence, key
@@ -298,6 +300,10 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 constexpr int kQsWarps = 4;
 constexpr int kQsCluster = 8;     // splits of a cluster
 constexpr int kQsMaxSplits = 64;  // of a sequence
+// Value scales (in the open block: values) from 2^(kQsRoom + 1) on raise the
+// unit that the output is summed in: 2^14 weights of 2^30 positions times 448
+// scales of less stay below 2^127.
+constexpr int kQsRoom = 72;
 
 template <int HDP>
 struct QsShape {
@@ -314,7 +320,7 @@ constexpr size_t qs_smem() {
   using S = QsShape<HDP>;
   return (size_t)(kQsWarps + 1) * 8 * NT * S::ORow * 4     // results of the warps and of the CTA
          + (size_t)S::KS * NT * QT * 32 * 8                // q
-         + (size_t)(8 * NT) * (3 + 2 * kQsWarps) * 4;      // row factors, m and l of the CTA and of the warps
+         + (size_t)(8 * NT) * (4 + 3 * kQsWarps) * 4;      // row factors; m, l and unit of the CTA and of the warps
 }
 
 // Splits of a sequence of `rows` rows a key head with `closed` positions in
@@ -412,8 +418,13 @@ __device__ __forceinline__ float4 ld_peer4(uint32_t a) {
   return v;
 }
 
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 // Weight of a partial result with maximum m under the total's maximum M.
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(m - M); }
+// The output of a row: O in units of 2^(X - 14), L the weights' sum; 0 where nothing is seen.
+__device__ __forceinline__ float row_result(float O, float L, int X) {
+  return L == 0.0f ? 0.0f : O / (L * 16384.0f) * pow2(X);
+}
 
 // EXACT: head_dim is HDP; else HDP is the next instantiated size and the
 // dims behind head_dim are zeros that are not read.
@@ -435,9 +446,10 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
   float* res = wo_all + kQsWarps * WO;                  // [ROWS][ORow]
   uint2* qf = reinterpret_cast<uint2*>(res + WO);
   float* fac = reinterpret_cast<float*>(qf + S::KS * NT * QT * 32);  // [ROWS] row factors
-  float* cm = fac + ROWS;                                             // [ROWS] the CTA's m, then l
-  float* wm = cm + 2 * ROWS;                                          // [warps][ROWS] m, then [warps][ROWS] l
+  float* cm = fac + ROWS;                                             // [ROWS] the CTA's m, then l, then unit
+  float* wm = cm + 3 * ROWS;                                          // [warps][ROWS] m, then l, then unit
   float* wl = wm + kQsWarps * ROWS;
+  int* wx = reinterpret_cast<int*>(wl + kQsWarps * ROWS);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, cq = lane & 3;
   const int csize = (int)cluster_size(), rank = (int)cluster_rank();
   // clusters are powers of two; the usual call has one group and one tile
@@ -607,6 +619,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 
     float o[MT][NT][4] = {};
     float m[NT][2], l[NT][2], f[NT][2];
+    int unit = 0;  // o is in units of 2^(unit - 14)
     int seen[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -619,6 +632,19 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
         seen[n][e] = x0 + x >= R ? 0 : a.causal ? len - (s.nrow - 1 - token_of(x0 + x)) : len;
       }
 
+    // exponent of a scale over kQsRoom; the same in the whole warp
+    auto unit_of_values = [](float v) { return (__float_as_int(v) >> 23) - 127 - kQsRoom; };
+    auto move_unit = [&](int to) {
+      if (to <= unit) return;
+      const float f = pow2(unit - to);
+      unit = to;
+#pragma unroll
+      for (int j = 0; j < MT; j++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[j][n][e] *= f;
+    };
     for (int it = 0; it < steps; it++) {
       const int t0 = t_first + it * S::UNIT;
       ahead(it + S::AHEAD);
@@ -661,25 +687,38 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
               if (hid || t >= seen[n][e & 1]) sc[g][n][e] = -INFINITY;
           }
       }
-      // ---- running maximum of weight times value scale, weights, their sum
+      // ---- the blocks' largest scores, the running maximum, weights, their sum
       uint32_t p[S::NG][NT][2][2];
-      float lam[S::NG];
+      float co[S::NG][NT][2];  // what a product of the block counts in the row's output
+      {
+        float big = vs[0];
 #pragma unroll
-      for (int g = 0; g < S::NG; g++) lam[g] = scale_exponent(vs[g]);
+        for (int g = 1; g < S::NG; g++) big = fmaxf(big, vs[g]);
+        if (big >= pow2(kQsRoom + 1)) move_unit(unit_of_values(big));
+      }
+      const float per_unit = pow2(-unit);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        float ref[2], al[2];
+        float mb[S::NG][2], al[2];
+#pragma unroll
+        for (int g = 0; g < S::NG; g++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float mx = fmaxf(sc[g][n][e], sc[g][n][e + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mb[g][e] = mx;
+          }
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          float mx = fmaxf(sc[0][n][e], sc[0][n][e + 2]) + lam[0];
+          float mn = m[n][e];
 #pragma unroll
-          for (int g = 1; g < S::NG; g++) mx = fmaxf(mx, fmaxf(sc[g][n][e], sc[g][n][e + 2]) + lam[g]);
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float mn = fmaxf(m[n][e], mx);
-          ref[e] = mn == -INFINITY ? 0.0f : mn;
-          al[e] = ex2(m[n][e] - ref[e]);
+          for (int g = 0; g < S::NG; g++) mn = fmaxf(mn, mb[g][e]);
+          const float ref = mn == -INFINITY ? 0.0f : mn;
+          al[e] = ex2(m[n][e] - ref);
           m[n][e] = mn;
+#pragma unroll
+          for (int g = 0; g < S::NG; g++) co[g][n][e] = ex2(mb[g][e] - ref);
         }
         if (__any_sync(0xffffffffu, !(al[0] == 1.0f && al[1] == 1.0f))) {
 #pragma unroll
@@ -690,19 +729,26 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
             for (int e = 0; e < 4; e++) o[j][n][e] *= al[e & 1];
         }
 #pragma unroll
-        for (int g = 0; g < S::NG; g++)
+        for (int g = 0; g < S::NG; g++) {
+          const float ref0 = mb[g][0] == -INFINITY ? 0.0f : mb[g][0], ref1 = mb[g][1] == -INFINITY ? 0.0f : mb[g][1];
+          float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {  // rows r, then r + 8
-            float p0 = ex2(sc[g][n][e] - ref[0]), p1 = ex2(sc[g][n][e + 1] - ref[1]);
-            l[n][0] += p0;
-            l[n][1] += p1;
-            p0 = p0 * vs[g] * 16384.0f;  // in this order: the scale of hidden positions may be near the largest number
-            p1 = p1 * vs[g] * 16384.0f;
+            float p0 = ex2(sc[g][n][e] - ref0), p1 = ex2(sc[g][n][e + 1] - ref1);
+            sum0 += p0;
+            sum1 += p1;
+            p0 *= 16384.0f;
+            p1 *= 16384.0f;
             const __half2 hi = __floats2half2_rn(p0, p1);
             p[g][n][0][e >> 1] = transpose8(h2_bits(hi));
             const float2 back = __half22float2(hi);
             p[g][n][1][e >> 1] = transpose8(h2_bits(__floats2half2_rn(p0 - back.x, p1 - back.y)));
           }
+          l[n][0] = fmaf(sum0, co[g][n][0], l[n][0]);
+          l[n][1] = fmaf(sum1, co[g][n][1], l[n][1]);
+          co[g][n][0] *= vs[g] * per_unit;
+          co[g][n][1] *= vs[g] * per_unit;
+        }
       }
       // ---- values
 #pragma unroll
@@ -720,16 +766,11 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
             const int j = 2 * v + h;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-              if constexpr (TYPE != kQ8F32) {
+              float d[4];
+              mma16816_zero(d, af, p[g][n][0][0], p[g][n][0][1]);
+              mma16816(d, af, p[g][n][1][0], p[g][n][1][1]);
 #pragma unroll
-                for (int q = 0; q < 2; q++) mma16816(o[j][n], af, p[g][n][q][0], p[g][n][q][1]);
-              } else {
-                float d[4];
-                mma16816_zero(d, af, p[g][n][0][0], p[g][n][0][1]);
-                mma16816(d, af, p[g][n][1][0], p[g][n][1][1]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[j][n][e] += d[e];
-              }
+              for (int e = 0; e < 4; e++) o[j][n][e] = fmaf(d[e], co[g][n][e & 1], o[j][n][e]);
             }
           }
         }
@@ -751,7 +792,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
         for (int e = 0; e < 4; e++) f[e] = E::to(x[e]);
       };
-      float lam[OPEN];  // exponent of a token's values: the same part as a block's scale
+      float lam[OPEN];  // a token's largest value
       bool there[OPEN];
 #pragma unroll
       for (int y = 0; y < OPEN; y++) {
@@ -774,7 +815,9 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
         for (int y = 0; y < OPEN; y++) lam[y] = fmaxf(lam[y], __shfl_xor_sync(0xffffffffu, lam[y], d));
 #pragma unroll
-      for (int y = 0; y < OPEN; y++) lam[y] = scale_exponent(lam[y]);
+      for (int y = 0; y < OPEN; y++)
+        if (lam[y] >= pow2(kQsRoom + 1)) move_unit(unit_of_values(lam[y]));
+      const float scale_up = pow2(14 - unit);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         float dot[OPEN];  // of row r, over the thread's dims
@@ -823,16 +866,16 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
         for (int e = 0; e < 2; e++) {
           float mn = m[n][e];
 #pragma unroll
-          for (int y = 0; y < OPEN; y++) mn = fmaxf(mn, w[y][e] + lam[y]);
+          for (int y = 0; y < OPEN; y++) mn = fmaxf(mn, w[y][e]);
           const float ref = mn == -INFINITY ? 0.0f : mn;
           al[e] = ex2(m[n][e] - ref);
-          m[n][e] = mn;
           l[n][e] *= al[e];
+          m[n][e] = mn;
 #pragma unroll
           for (int y = 0; y < OPEN; y++) {
             w[y][e] = ex2(w[y][e] - ref);
             if (r == 0) l[n][e] += w[y][e];
-            w[y][e] *= 16384.0f;
+            w[y][e] *= scale_up;
           }
         }
 #pragma unroll
@@ -871,6 +914,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
         if (r == 0) {
           wm[warp * ROWS + row] = m[n][e];
           wl[warp * ROWS + row] = x;
+          wx[warp * ROWS + row] = unit;
         }
 #pragma unroll
         for (int j = 0; j < MT; j++)
@@ -882,15 +926,20 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
     for (int x = tid; x < rows * (HDP / 4); x += kQsWarps * 32) {
       const int row = x / (HDP / 4), d = x % (HDP / 4) * 4;
       float M = -INFINITY;
+      int X = 0;
 #pragma unroll
-      for (int w = 0; w < kQsWarps; w++) M = fmaxf(M, wm[w * ROWS + row]);
+      for (int w = 0; w < kQsWarps; w++) {
+        M = fmaxf(M, wm[w * ROWS + row]);
+        X = max(X, wx[w * ROWS + row]);
+      }
       float L = 0.0f, O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < kQsWarps; w++) {
-        const float wt = part_weight(wm[w * ROWS + row], M);
+        float wt = part_weight(wm[w * ROWS + row], M);
         const float4 y = *reinterpret_cast<const float4*>(wo_all + w * WO + row * S::ORow + d);
         // a warp whose maximum is -inf holds zeros, or NaN from a NaN score
         L = fmaf(wt, wl[w * ROWS + row], L);
+        wt *= pow2(wx[w * ROWS + row] - X);
         O[0] = fmaf(wt, y.x, O[0]);
         O[1] = fmaf(wt, y.y, O[1]);
         O[2] = fmaf(wt, y.z, O[2]);
@@ -900,6 +949,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
       if (d == 0) {
         cm[row] = M;
         cm[ROWS + row] = L;
+        cm[2 * ROWS + row] = __int_as_float(X);
       }
     }
     // ---- merge of the splits, in order; the rows' dims are dealt out over the cluster
@@ -911,16 +961,22 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
         const int row = x / (HDP / 4), d = x % (HDP / 4) * 4;
         if (d >= hd) continue;
         float L, M, O[4];
+        int X;
         if (ns > 1) {
           M = -INFINITY;
+          X = 0;
 #pragma unroll 4
-          for (int q = 0; q < ns; q++) M = fmaxf(M, ld_peer(peer_addr(cm_u + row * 4, q)));
+          for (int q = 0; q < ns; q++) {
+            M = fmaxf(M, ld_peer(peer_addr(cm_u + row * 4, q)));
+            X = max(X, __float_as_int(ld_peer(peer_addr(cm_u + (2 * ROWS + row) * 4, q))));
+          }
           L = O[0] = O[1] = O[2] = O[3] = 0.0f;
 #pragma unroll 4
           for (int q = 0; q < ns; q++) {
-            const float wt = part_weight(ld_peer(peer_addr(cm_u + row * 4, q)), M);
+            float wt = part_weight(ld_peer(peer_addr(cm_u + row * 4, q)), M);
             const float4 y = ld_peer4(peer_addr(res_u + (row * S::ORow + d) * 4, q));
             L = fmaf(wt, ld_peer(peer_addr(cm_u + (ROWS + row) * 4, q)), L);
+            wt *= pow2(__float_as_int(ld_peer(peer_addr(cm_u + (2 * ROWS + row) * 4, q))) - X);
             O[0] = fmaf(wt, y.x, O[0]);
             O[1] = fmaf(wt, y.y, O[1]);
             O[2] = fmaf(wt, y.z, O[2]);
@@ -929,6 +985,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
         } else {
           M = cm[row];
           L = cm[ROWS + row];
+          X = __float_as_int(cm[2 * ROWS + row]);
 #pragma unroll
           for (int e = 0; e < 4; e++) O[e] = res[row * S::ORow + d + e];
         }
@@ -939,13 +996,13 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
           if (d == 0) {
             y[hd] = M;
             y[hd + 1] = L;
+            y[hd + 2] = __int_as_float(X);
           }
           continue;
         }
-        // O is 2^14 sum p v, L is sum p; nothing seen: L = 0
         T* y = out0 + (int64_t)token * a.out.token + (int64_t)head * a.out.head + d;
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = E::from(L == 0.0f ? 0.0f : O[e] / (L * 16384.0f));
+        for (int e = 0; e < 4; e++) y[e] = E::from(row_result(O[e], L, X));
       }
     }
     if (csize > 1) cluster_arrive_wait();  // peers are done with this CTA's result
@@ -985,15 +1042,20 @@ __global__ void __launch_bounds__(128) k_q8_merge(Q8View c, Q8Batch b, Q8Attend 
   const int n = (splits + kQsCluster - 1) / kQsCluster;
   const float* y = a.ws + (size_t)w * groups * (c.hd + 4);
   float M = -INFINITY;
-  for (int g = 0; g < n; g++) M = fmaxf(M, y[g * (c.hd + 4) + c.hd]);
+  int X = 0;
+  for (int g = 0; g < n; g++) {
+    M = fmaxf(M, y[g * (c.hd + 4) + c.hd]);
+    X = max(X, __float_as_int(y[g * (c.hd + 4) + c.hd + 2]));
+  }
   for (int d = lane * 4; d < c.hd; d += 128) {
     float L = 0.0f, O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int g = 0; g < n; g++) {
       const float* z = y + g * (c.hd + 4);
-      const float wt = part_weight(z[c.hd], M);
+      float wt = part_weight(z[c.hd], M);
       const float4 x = *reinterpret_cast<const float4*>(z + d);
       L = fmaf(wt, z[c.hd + 1], L);
+      wt *= pow2(__float_as_int(z[c.hd + 2]) - X);
       O[0] = fmaf(wt, x.x, O[0]);
       O[1] = fmaf(wt, x.y, O[1]);
       O[2] = fmaf(wt, x.z, O[2]);
@@ -1001,7 +1063,7 @@ __global__ void __launch_bounds__(128) k_q8_merge(Q8View c, Q8Batch b, Q8Attend 
     }
     T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)token * a.out.token + (int64_t)head * a.out.head + d;
 #pragma unroll
-    for (int e = 0; e < 4; e++) out[e] = E::from(L == 0.0f ? 0.0f : O[e] / (L * 16384.0f));
+    for (int e = 0; e < 4; e++) out[e] = E::from(row_result(O[e], L, X));
   }
 }
 

@@ -3,11 +3,16 @@
 // cores, 16-bit caches with head_dim up to 128.
 //
 // Mathematics: the one of k_q8_attend (q8.cu) at this size. Codes are exact
-// fp16 operands; a q row is scaled by a power of two into fp16; the weights
-// carry the value scales, P' = 2^(x + log2 s_V - m), with a reference m that
-// follows the maximum of x + floor(log2 s_V) and is moved only when that has
-// grown by 2^8 (P' is held times 2^6, so it stays below 2^15): the output is
-// rescaled a few times a row instead of at every tile. The tokens of the open
+// fp16 operands; a q row is scaled by a power of two into fp16. The products
+// with the values stay in tensor memory from block to block, so the weights
+// carry the value scales: P' = 2^(x - m) s_V 2^(10 - D), where m follows the
+// maximum of the scores x and m + D that of x + floor(log2 s_V). m is moved
+// when the maximum has grown by 2^16, D when the other one has by 2^4 (P' stays
+// below 2^15): the output is rescaled a few times a row instead of at every
+// tile. The sum of the weights is relative to m alone, so no size of the values
+// takes bits from it. A weight ends at 2^-25, 2^-35 of the row's largest weight
+// times value scale: where one block's values are 2^20 times the others', those
+// keep 15 bits, where they are 2^30 times, 5. The tokens of the open
 // block are 16-bit numbers: scaled by a power of two for the block they are
 // fp16 operands like codes (an element 2^30 times smaller than the block's
 // largest loses bits). Weights are two fp16 terms (22 bits). Output and sums stay
@@ -48,13 +53,18 @@ constexpr int kQtM = 128;          // rows of a tile
 constexpr int kQtN = 128;          // positions of a block
 constexpr int kQtThreads = 17 * 32;
 constexpr int kQtSlots = 4;        // ring of scales and masks
+// A weight's operand is 2^(x - m) s_V 2^(kQtUnit - D), where x + log2 s_V is at
+// most m + D + kQtLagD + 1: below 2^15.
+constexpr int kQtUnit = 10;
+constexpr float kQtLagD = 4.0f, kQtLagM = 16.0f;
+constexpr float kQtLeast = -100.0f;  // D of a row that has seen nothing; scale_exponent's least
 constexpr unsigned long long kQtWaitNs = 2000000000ull;
 
 // Scales and masks of one block of positions.
 struct QtScales {
   float ks[kQtN / kQ8Block];    // K scale
-  float vs64[kQtN / kQ8Block];  // V scale times 2^6
-  float lam[kQtN / kQ8Block];   // exponent of the V scale
+  float vs[kQtN / kQ8Block];    // V scale
+  float lam[kQtN / kQ8Block];   // its exponent
   uint32_t show[kQtN / 32];     // bit per position: exists and is not hidden
 };
 
@@ -354,7 +364,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
 
       const uint32_t ts = tm_s[wg] + ((uint32_t)((warp & 3) * 32) << 16);
       const uint32_t to = tm_o[wg] + ((uint32_t)((warp & 3) * 32) << 16);
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f, D = kQtLeast;  // references of the scores and of their products with values
       bool ok = true;
       for (int t = 0; t < nb; t++) {
         const unsigned blk = n_sc + t;
@@ -383,8 +393,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         // scores (below 2^30) times this least one are 0 to every bit that counts.
         auto scale_of = [&](int g) { return fmaxf(sc.ks[g] * fs, 1.0e-36f); };
         uint32_t z[2][16];  // one part is worked on while the next one comes
-        // ---- the largest score with its value scale
-        float mx = -INFINITY;
+        // ---- the largest score mx, and the largest score with its value scale, mx + dx
+        float mx = m, dx = D;
         tm_ld16(z[0], ts);
 #pragma unroll 2
         for (int g = 0; g < kQtN / 16; g++) {
@@ -396,17 +406,23 @@ __global__ void __launch_bounds__(kQtThreads, 1)
 #pragma unroll
           for (int e = 1; e < 15; e += 2) y = max3(y, __uint_as_float(w[e]), __uint_as_float(w[e + 1]));
           y = fmaxf(y, __uint_as_float(w[15]));
-          mx = fmaxf(mx, fmaf(y, scale_of(g), sc.lam[g]));
+          y *= scale_of(g);
+          const float old = mx;
+          mx = fmaxf(mx, y);
+          const float at = mx == -INFINITY ? 0.0f : mx;
+          dx = fmaxf(dx + (old - at), sc.lam[g] + (y - at));
         }
-        // ---- move the reference when it has fallen far behind
-        if (t == 0) {
-          m = mx;
-        } else {
-          const bool move = mx > m + 8.0f;
-          if (__any_sync(0xffffffffu, move)) {
-            const float al = move ? ex2(m - mx) : 1.0f;
-            if (move) m = mx;
-            l *= al;
+        // ---- move the references when one has fallen far behind
+        const bool move = mx > m + kQtLagM || dx + (mx - m) > D + kQtLagD;  // m of -inf: whenever mx is more
+        const float dn = fmaxf(ceilf(dx), kQtLeast);
+        if (__any_sync(0xffffffffu, move)) {
+          const float al = move ? ex2((m - mx) + (D - dn)) : 1.0f;
+          if (move) {
+            l *= ex2(m - mx);
+            m = mx;
+            D = dn;
+          }
+          if (t) {
 #pragma unroll 1
             for (int j = 0; j < HDT / 32; j++) {
               uint32_t w[32];
@@ -419,7 +435,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
             tm_wait_st();
           }
         }
-        const float ref = m == -INFINITY ? 0.0f : m;
+        const float ref = m == -INFINITY ? 0.0f : m, unit = exp2i(kQtUnit - (int)D);
+        const bool far = __any_sync(0xffffffffu, fabsf(ref) > 1.0e6f);
         // ---- weights over the scores
         const uint64_t nref = f2(-ref, -ref);
         uint64_t l2 = f2(0.0f, 0.0f);
@@ -429,8 +446,15 @@ __global__ void __launch_bounds__(kQtThreads, 1)
           tm_wait(w);
           if (g + 1 < kQtN / 16) tm_ld16(z[(g + 1) & 1], ts + (g + 1) * 16);
           cover(w, g * 16);
-          const float cs = scale_of(g), vs = sc.vs64[g];
-          const uint64_t cs2 = f2(cs, cs), vs2 = f2(vs, vs);
+          const float cs = scale_of(g), vs = fminf(sc.vs[g] * unit, FLT_MAX);  // beyond that the weights are 0
+          uint64_t cs2 = f2(cs, cs), vs2 = f2(vs, vs);
+          if (far) {
+            // products rounded as the reference was: what a fused step leaves of their
+            // rounding is no longer small
+#pragma unroll
+            for (int e = 0; e < 16; e++) w[e] = __float_as_uint(__uint_as_float(w[e]) * cs);
+            cs2 = f2(1.0f, 1.0f);
+          }
           uint32_t p[16];  // the weights of 16 positions: 8 words of the first terms, 8 of the second ones
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
@@ -459,7 +483,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       if (ok && nb) ok = __all_sync(0xffffffffu, qb_wait(&S.o_full[wg], n_q & 1, failed));
       if (nb) n_q++;
       T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)token * a.out.token + (int64_t)head * a.out.head;
-      const float inv = l == 0.0f ? 0.0f : __fdiv_rn(0.015625f, l);
+      const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l), back = exp2i((int)D - kQtUnit);
       qt_after();
 #pragma unroll 1
       for (int j = 0; j < HDT / 32; j++) {
@@ -487,7 +511,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         __align__(16) T y[32];
         const bool zero = ok && l == 0.0f;  // nothing seen
 #pragma unroll
-        for (int e = 0; e < 32; e++) y[e] = E::from(zero ? 0.0f : __uint_as_float(v[e]) * (ok ? inv : 1.0f));
+        for (int e = 0; e < 32; e++) y[e] = E::from(zero ? 0.0f : __uint_as_float(v[e]) * (ok ? inv : 1.0f) * back);
         if (a.out_aligned) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
@@ -632,7 +656,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
               vs = open_v;
             }
             sc.ks[ct] = ks;
-            sc.vs64[ct] = vs * 64.0f;
+            sc.vs[ct] = vs;
             sc.lam[ct] = scale_exponent(vs);
           }
           qb_arrive(&S.sc_full[n % kQtSlots]);

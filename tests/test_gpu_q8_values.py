@@ -59,3 +59,40 @@ def test_weights_keep_more_bits_than_the_result(dtype, kind, rows, heads, kvh, h
     c = Case(4, kvh, 352, hd, kind, dtype, seed=hd + rows)
     c.append([0, 1, 2, 3], [150, 40, 345, 208])
     check(c, [2, 0, 3, 1], rows, heads)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 140])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_values_near_the_largest_number(dtype, kind, rows, hd):
+    c = Case(5, 1, 192, hd, kind, dtype, seed=9)
+    lens = [1, 10, 160, 171, 175]
+    # the tiles hold a block's values as 16-bit numbers in units of its largest: no dims 2^40 below it
+    tiles = on_tiles(dtype, hd, rows, 4)
+    v = c.randn(sum(lens), 1, hd)
+    v[0] = v[0] * 1e37 if tiles else v[0]
+    v[0, 0, 7] = 2e38                                            # alone
+    v[1:11] = (v[1:11].float().clamp(-3, 3) * 1e38).to(dtype)    # the open block alone
+    v[11:171] = (v[11:171].float().clamp(-3, 3) * 1e38).to(dtype)  # closed blocks alone
+    at = 171
+    v[at + 165, 0, 3] = 3e38                                     # one in the open block, ordinary ones before it
+    at += 171
+    v[at:at + 175] = (v[at:at + 175].float().clamp(-3, 3) * 1e38).to(dtype)
+    c.append([0, 1, 2, 3, 4], lens, c.randn(sum(lens), 1, hd), v)
+    out = check(c, [0, 1, 2, 4] if tiles else [0, 1, 2, 3, 4], rows, 4, causal=False)
+    assert torch.isfinite(out).all()
+    check(c, [4, 2], rows, 4)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 20, 140])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("where", [50, 171])
+def test_one_value_that_dwarfs_the_others_leaves_their_dims_alone(dtype, rows, hd, where):
+    """`where`: a closed block, the open one. 1e9 times the others (the tiles: 2^14 times)."""
+    c = Case(1, 2, 192, hd, "int8", dtype, seed=10)
+    k, v = c.randn(174, 2, hd), c.randn(174, 2, hd)
+    v[where, :, 5] = 2.0 ** 14 if on_tiles(dtype, hd, rows, 2) else 1e9
+    c.append([0], [174], k, v)
+    check(c, [0], rows, 4, causal=False)
