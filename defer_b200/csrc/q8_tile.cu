@@ -13,10 +13,12 @@
 // takes bits from it. A weight ends at 2^-25, 2^-35 of the row's largest weight
 // times value scale: where one block's values are 2^20 times the others', those
 // keep 15 bits, where they are 2^30 times, 5. The tokens of the open
-// block are 16-bit numbers: scaled by a power of two for the block they are
-// fp16 operands like codes (an element 2^30 times smaller than the block's
-// largest loses bits). Weights are two fp16 terms (22 bits). Output and sums stay
-// in fp32 (tensor memory, registers).
+// block are 16-bit numbers: scaled by a power of two for the block, its largest
+// element to 2^15 or more, they are fp16 operands like codes. fp16 tokens lose
+// no bit by that; of a bf16 token, an element 2^32 times smaller than the
+// block's largest begins to (fp16 numbers end at 2^-24), as does an element of
+// a bf16 q row 2^31 times smaller than the row's largest. Weights are two fp16
+// terms (22 bits). Output and sums stay in fp32 (tensor memory, registers).
 //
 // Work: a CTA takes two tiles of 128 rows (rows of the heads that share a key
 // head, token after token), so that a converted block of 128 positions feeds
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
             if (!(w >> e & 1)) v[e] = 0xff800000u;
         };
         // Scale of a block's scores: never 0, which would turn -inf into NaN;
-        // scores (below 2^30) times this least one are 0 to every bit that counts.
+        // scores (below 2^38) times this least one are 0 to every bit that counts.
         auto scale_of = [&](int g) { return fmaxf(sc.ks[g] * fs, 1.0e-36f); };
         uint32_t z[2][16];  // one part is worked on while the next one comes
         // ---- the largest score mx, and the largest score with its value scale, mx + dx
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     const float* ksc = c.ks + sh * (c.cap / kQ8Block);
     const float* vsc = c.vs + sh * (c.cap / kQ8Block);
     float open_k, open_v;
-    {  // the open block's power-of-two scales: its largest finite element that is not hidden becomes [2^6, 2^7)
+    {  // the open block's power-of-two scales: its largest finite element that is not hidden becomes [2^15, 2^16)
       float ak = 0.0f, av = 0.0f;
       bool odd = false;
       for (int x = ct; x < (len - closed) * hd; x += 128) {
@@ -571,8 +573,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       const float mk = fmaxf(fmaxf(rk[0], rk[1]), fmaxf(rk[2], rk[3]));
       const float mv = fmaxf(fmaxf(rv[0], rv[1]), fmaxf(rv[2], rv[3]));
       // exponents from -96: smaller blocks keep fewer than their own bits
-      open_k = mk > 0.0f ? exp2i(max(exponent_of(mk), -96) - 6) : 1.0f;
-      open_v = mv > 0.0f ? exp2i(max(exponent_of(mv), -96) - 6) : 1.0f;
+      open_k = mk > 0.0f ? exp2i(max(exponent_of(mk), -96) - 15) : 1.0f;
+      open_v = mv > 0.0f ? exp2i(max(exponent_of(mv), -96) - 15) : 1.0f;
       const int* ro = S.red_odd[is_v];
       if (ct == 0 && !is_v) S.open_odd = ro[0] | ro[1] | ro[2] | ro[3];
     }

@@ -96,3 +96,18 @@ def test_one_value_that_dwarfs_the_others_leaves_their_dims_alone(dtype, rows, h
     v[where, :, 5] = 2.0 ** 14 if on_tiles(dtype, hd, rows, 2) else 1e9
     c.append([0], [174], k, v)
     check(c, [0], rows, 4, causal=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows", [1, 140])
+def test_small_elements_of_the_open_block(dtype, rows):
+    """Elements 2^16 to 2^24 below the largest of the open block keep their bits."""
+    for hd in (64, 128):
+        c = Case(1, 1, 32, hd, "int8", dtype, seed=11)
+        v = c.randn(13, 1, hd).float()
+        v = v.clamp(-3, 3) * torch.exp2(-(torch.arange(hd, device="cuda") % 9).float())
+        v = v * 2.0 ** -3
+        v[4, 0, 0] = 2.0 ** 13
+        k = c.randn(13, 1, hd)
+        c.append([0], [13], k, v.to(dtype))
+        check(c, [0], rows, 2, causal=False)
