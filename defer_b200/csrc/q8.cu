@@ -320,7 +320,7 @@ constexpr size_t qs_smem() {
   using S = QsShape<HDP>;
   return (size_t)(kQsWarps + 1) * 8 * NT * S::ORow * 4     // results of the warps and of the CTA
          + (size_t)S::KS * NT * QT * 32 * 8                // q
-         + (size_t)(8 * NT) * (4 + 3 * kQsWarps) * 4;      // row factors; m, l and unit of the CTA and of the warps
+         + (size_t)(8 * NT) * (6 + 3 * kQsWarps) * 4;      // row factors; m, l and unit of the CTA and of the warps
 }
 
 // Splits of a sequence of `rows` rows a key head with `closed` positions in
@@ -446,7 +446,9 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
   float* res = wo_all + kQsWarps * WO;                  // [ROWS][ORow]
   uint2* qf = reinterpret_cast<uint2*>(res + WO);
   float* fac = reinterpret_cast<float*>(qf + S::KS * NT * QT * 32);  // [ROWS] row factors
-  float* cm = fac + ROWS;                                             // [ROWS] the CTA's m, then l, then unit
+  float* q_down = fac + ROWS;                                         // [ROWS] the power of two that q was raised by
+  float* q_rest = q_down + ROWS;                                      // [ROWS] the rest of fac
+  float* cm = q_rest + ROWS;                                          // [ROWS] the CTA's m, then l, then unit
   float* wm = cm + 3 * ROWS;                                          // [warps][ROWS] m, then l, then unit
   float* wl = wm + kQsWarps * ROWS;
   int* wx = reinterpret_cast<int*>(wl + kQsWarps * ROWS);
@@ -597,8 +599,12 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
       // applied in two steps: 2^up itself may exceed fp32's range.
       const int up = mx > 0.0f && mx <= FLT_MAX ? 141 - (__float_as_int(mx) >> 23) : 0;  // -113 .. 141
       const float up0 = __int_as_float((127 + up / 2) << 23), up1 = __int_as_float((127 + up - up / 2) << 23);
-      if (lane == 0)
-        fac[x] = a.scale * 1.4426950408889634f * __int_as_float((127 - up / 2) << 23) * __int_as_float((127 - up + up / 2) << 23);
+      if (lane == 0) {
+        const float f = a.scale * 1.4426950408889634f;
+        fac[x] = f * __int_as_float((127 - up / 2) << 23) * __int_as_float((127 - up + up / 2) << 23);
+        q_down[x] = pow2(max(-up, -126));
+        q_rest[x] = f * pow2(min(126 - up, 0));
+      }
 #pragma unroll
       for (int e = 0; e < HDP / 32; e++) {
         const int d = e * 32 + lane;
@@ -826,7 +832,8 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
 #pragma unroll
         for (int k = 0; k < S::KS; k++) {
           const int d0 = HDP >= 64 ? (k / 4 * 4 + cq) * 16 + k % 4 * 4 : cq * 8 + k * 4;
-          float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // in its own size: raised, its products with large keys would overflow
+          const float down = q_down[n * 8 + r];
 #pragma unroll
           for (int x = QT - 1; x >= 0; x--) {
             const uint2 bf = qf[((k * NT + n) * QT + x) * 32 + lane];
@@ -837,6 +844,8 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
             q[2] += hi.x;
             q[3] += hi.y;
           }
+#pragma unroll
+          for (int e = 0; e < 4; e++) q[e] *= down;
           if (EXACT || d0 < hd) {
 #pragma unroll
             for (int y = 0; y < OPEN; y++)
@@ -854,7 +863,7 @@ __global__ void __launch_bounds__(kQsWarps * 32, HDP == 256 || NT == 2 ? 2 : 4)
         for (int y = 0; y < OPEN; y++) {
           dot[y] += __shfl_xor_sync(0xffffffffu, dot[y], 1);
           dot[y] += __shfl_xor_sync(0xffffffffu, dot[y], 2);
-          dot[y] *= fac[n * 8 + r];
+          dot[y] *= q_rest[n * 8 + r];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const float x = __shfl_sync(0xffffffffu, dot[y], (2 * cq + e) * 4);

@@ -111,3 +111,23 @@ def test_small_elements_of_the_open_block(dtype, rows):
         k = c.randn(13, 1, hd)
         c.append([0], [13], k, v.to(dtype))
         check(c, [0], rows, 2, causal=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 140])
+@pytest.mark.parametrize("at", [20, 166])
+def test_keys_near_the_largest_number(dtype, rows, at):
+    """Scores far beyond what an exponential can hold: the largest one's value, whatever the values' size."""
+    for size in (1.0, 1e6, 1e30):
+        c = Case(1, 1, 192, 64, "int8", dtype, seed=12)
+        k, v = c.randn(170, 1, 64), (c.randn(170, 1, 64).float() * size).to(dtype)
+        k[at, 0, 2] = 1e35
+        c.append([0], [170], k, v)
+        q = c.randn(rows, 2, 64)
+        q[..., 2] = 1.0
+        out = torch.empty_like(q)
+        D.q8_attend(c.cache, q, out, ints([170]), causal=False)
+        want = torch.tensor(c.values(0)[1][0, at], device="cuda").to(dtype)
+        step = torch.finfo(dtype).eps
+        bad = ((out - want).abs() > step * want.abs()) | torch.isnan(out)
+        assert bad.sum().item() == 0, (size, out[0, 0, :4].tolist(), want[:4].tolist())
