@@ -18,6 +18,7 @@
 
 #include "common.h"
 #include "q8.cuh"
+#include "smem.h"
 
 namespace defer {
 namespace {
@@ -1142,24 +1143,12 @@ void q8_read(const Q8View& c, int n, const int* lens, const int* start, const in
 
 namespace {
 
-// Kernel attributes are set once per device.
-bool first_on_device(unsigned long long& mask) {
-  int dev = 0;
-  DEFER_CUDA(cudaGetDevice(&dev));
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (mask & bit) return false;
-  mask |= bit;
-  return true;
-}
-
 template <int TYPE, int KIND, int HDP, int NT, bool EXACT>
 void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st) {
   auto kern = k_q8_attend<TYPE, KIND, HDP, NT, EXACT>;
   constexpr size_t smem = qs_smem<HDP, NT, TYPE == kQ8F32 ? 2 : 1>();
-  static unsigned long long attr = 0;
-  if (first_on_device(attr)) {
-    DEFER_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  }
+  static SmemLimit limit;
+  limit.ensure([&] { SmemLimit::allow(kern, smem); });
   int64_t rows = (int64_t)std::max(b.max_q, 1) * (a.heads / c.kvh);
   if (a.tiled) rows = std::min<int64_t>(rows, kQ8FewRows);
   const int64_t tiles = std::min<int64_t>((rows + 8 * NT - 1) / (8 * NT), 65535 / c.kvh);

@@ -47,6 +47,7 @@
 
 #include "common.h"
 #include "q8.cuh"
+#include "smem.h"
 
 namespace defer {
 namespace {
@@ -753,13 +754,8 @@ void attend_tiles(const Q8View& c, const Q8Batch& b, const Q8Attend& a, int sms,
   auto kern = k_q8_tile<TYPE, KIND, HDT>;
   // all of tensor memory is taken, so one CTA an SM: with more than half of its shared memory too
   constexpr int smem = std::max((int)sizeof(QtShared<HDT>), 120 * 1024);
-  static unsigned long long attr = 0;
-  int dev = 0;
-  DEFER_CUDA(cudaGetDevice(&dev));
-  if (!(attr >> (dev & 63) & 1)) {
-    DEFER_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attr |= 1ull << (dev & 63);
-  }
+  static SmemLimit limit;
+  limit.ensure([&] { SmemLimit::allow(kern, smem); });
   // One tile a CTA while there are SMs for all of them, else two.
   const int64_t rows = (int64_t)std::max(b.max_q, 1) * (a.heads / c.kvh);
   const int64_t single = (rows + kQtM - 1) / kQtM;

@@ -53,6 +53,7 @@
 #include "common.h"
 #include "kernels.h"
 #include "phases.cuh"
+#include "smem.h"
 #include "tc.h"
 
 namespace defer {
@@ -619,22 +620,10 @@ int tc_splits(const TcMatrix& w, int sms) {
   return std::max(1, std::min({sms / std::max(1, w.ntile), w.nkb / 4, best}));
 }
 
-// Kernel attributes are set once per device.
-static bool first_on_device(unsigned long long& mask) {
-  int dev = 0;
-  DEFER_CUDA(cudaGetDevice(&dev));
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (mask & bit) return false;
-  mask |= bit;
-  return true;
-}
-
 void tc_gemm(const unsigned char* A, const TcMatrix& w, float* Y, int splits, unsigned* tickets, int* status,
              cudaStream_t s, const int* active) {
-  static unsigned long long attr = 0;
-  if (first_on_device(attr))
-    DEFER_CUDA(cudaFuncSetAttribute(k_tc_gemm, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    kTcStages * kTcStageMax));
+  static SmemLimit limit;
+  limit.ensure([] { SmemLimit::allow(k_tc_gemm, kTcStages * kTcStageMax); });
   const int smem = kTcStages * (tc_aterms(w) * kTcABytes + w.wterms * kTcWBytes);
   TcGemmArgs g;
   g.A = A;
@@ -663,12 +652,12 @@ static void steps_tc(const DModel& m, const TcModel& tm, const DBatch& bt0, int 
   const size_t smem = step_smem_bytes(m, bt.B, bt.max_chunks);
   bt.smem_bytes = (unsigned)smem;
   bt.parts = 1;
-  static unsigned long long attr = 0;
-  if (first_on_device(attr)) {
-    DEFER_CUDA(cudaFuncSetAttribute(k_tc_select<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    DEFER_CUDA(cudaFuncSetAttribute(k_tc_select<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    DEFER_CUDA(cudaFuncSetAttribute(k_tc_attn, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-  }
+  static SmemLimit limit;
+  limit.ensure([] {
+    SmemLimit::allow(k_tc_select<true>, 200 * 1024);
+    SmemLimit::allow(k_tc_select<false>, 200 * 1024);
+    SmemLimit::allow(k_tc_attn, 200 * 1024);
+  });
   if (smem > 200 * 1024) fail(kInvalidArgument, "tensor-core step: phase shared memory too large");
   const int attn_units = bt.B * m.NKV * bt.max_chunks;
   const int ew = std::min(sms * 8, 4096);  // epilogue grid

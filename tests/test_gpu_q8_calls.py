@@ -1,7 +1,12 @@
 """8-bit key/value cache on the GPU: calls that the documentation allows beside
 the ordinary ones (launch sizes, threads, streams, workspaces)."""
+import os
+import subprocess
+import sys
+
 import pytest
 
+from tests.conftest import ROOT
 from tests.test_gpu_q8 import Case, ints
 from tests.test_gpu_q8_values import check
 
@@ -22,3 +27,51 @@ def test_a_max_q_below_the_rows(dtype, hd, length, causal):
     start = ints([0, rows, 2 * rows])
     for max_q in (40, 200):
         check(c, [0, 1], rows, 2, causal=causal, q_start=start, max_q=max_q)
+
+
+FIRST_CALLS = """
+import threading
+import torch
+import defer_b200 as D
+
+refused = []
+torch.zeros(1, device="cuda")
+
+def first_call(kind, dtype, hd, rows, start):
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        z = lambda *s, dt: torch.zeros(*s, dtype=dt, device="cuda")
+        c = D.Q8Cache(z(1, 1, 32, hd, dt=kind), z(1, 1, 32, hd, dt=kind), z(1, 1, 2, dt=torch.float32),
+                      z(1, 1, 2, dt=torch.float32), z(1, 1, 16, hd, dt=dtype), z(1, 1, 16, hd, dt=dtype))
+        q = z(rows, 1, hd, dt=dtype)
+        out = torch.empty_like(q)
+        lens = torch.full((1,), 5, dtype=torch.int32, device="cuda")
+        st.synchronize()
+        start.wait()
+        try:
+            D.q8_attend(c, q, out, lens)
+        except D.DeferError as e:
+            refused.append((str(kind), hd, rows, str(e)))
+        st.synchronize()
+
+# kernels that need more shared memory than a launch gets unasked
+for kind in (torch.int8, torch.float8_e4m3fn):
+    for dtype, hd, rows in ((torch.float32, 256, 1), (torch.float32, 128, 12), (torch.float32, 80, 12),
+                            (torch.bfloat16, 128, 100), (torch.bfloat16, 64, 100)):
+        start = threading.Barrier(8)
+        ts = [threading.Thread(target=first_call, args=(kind, dtype, hd, rows, start)) for _ in range(8)]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+print(refused)
+assert not refused
+"""
+
+
+def test_first_calls_of_several_threads():
+    """A process of its own, whose threads make their first calls at the same moment."""
+    for _ in range(3):
+        r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, env={**os.environ, "PYTHONPATH": ROOT},
+                           capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stdout + r.stderr[-2000:]
