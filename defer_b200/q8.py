@@ -229,10 +229,14 @@ def _workspace_bytes(cache: Q8Cache, batch: bytes, max_len: int, heads: int) -> 
     return n.value
 
 
-def workspace_bytes(cache: Q8Cache, tokens: int, heads: int, max_len: int = 0) -> int:
-    """Bytes of workspace that q8_attend of `tokens` rows of `heads` heads
-    uses with this max_len (defer_q8_attend_workspace)."""
-    return _workspace_bytes(cache, _BATCH.pack(1, tokens, 0, 0, 0, 0), max_len, heads)
+def workspace_bytes(cache: Q8Cache, tokens: int, heads: int, max_len: int = 0, *, n: Optional[int] = None) -> int:
+    """Bytes of workspace with which q8_attend of `tokens` rows of `heads`
+    heads and this max_len runs, however the rows belong to sequences; with
+    `n`, of a call without q_start whose n sequences have tokens / n rows each
+    (defer_q8_attend_workspace; many rows a sequence need none)."""
+    # the host only asks whether there is a q_start: with one, sequences may have any number of rows
+    b = _BATCH.pack(1, tokens, 0, 1, 0, 0) if n is None else _BATCH.pack(n, tokens, 0, 0, 0, 0)
+    return _workspace_bytes(cache, b, max_len, heads)
 
 
 def _scratch(device: int, nbytes: int, stream: int):

@@ -6,6 +6,7 @@ import sys
 
 import pytest
 
+import defer_b200 as D
 from tests.conftest import ROOT
 from tests.test_gpu_q8 import Case, ints
 from tests.test_gpu_q8_values import check
@@ -75,3 +76,27 @@ def test_first_calls_of_several_threads():
         r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, env={**os.environ, "PYTHONPATH": ROOT},
                            capture_output=True, text=True, timeout=300)
         assert r.returncode == 0, r.stdout + r.stderr[-2000:]
+
+
+def test_a_workspace_of_the_size_that_is_named():
+    """64 sequences of one row, and ragged ones, over more than one cluster's splits."""
+    n, length = 64, 9600
+    c = Case(n, 2, length, 128, "int8", BF16)
+    for x in c.codes:
+        x.zero_()
+    for x in (*c.scales, *c.tails):
+        x.zero_()
+    q = c.randn(n, 16, 128)
+    lens = ints([length - 150 * i for i in range(n)])
+    need = D.q8.workspace_bytes(c.cache, n, 16, length)
+    assert need
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, 77.0)
+    D.q8_attend(c.cache, q, out, lens, max_len=length, workspace=ws)
+    assert (out == 0).all()  # the values are zeros
+    out.fill_(77.0)
+    D.q8_attend(c.cache, q, out, lens[:3].contiguous(), q_start=ints([0, 1, 40, n]), slots=ints([5, 6, 7]), max_q=39,
+                max_len=length, workspace=ws)
+    assert (out == 0).all()
+    with pytest.raises(D.InvalidArgumentError, match="workspace"):
+        D.q8_attend(c.cache, q, out, lens, max_len=length, workspace=ws[:need - 16])
