@@ -245,5 +245,7 @@ def _scratch(device: int, nbytes: int, stream: int):
         _refuse("a sequence this long needs the workspace argument")
     if stream == t.cuda.current_stream(device).cuda_stream:
         return t.empty(nbytes, dtype=t.uint8, device=f"cuda:{device}")
-    with t.cuda.stream(t.cuda.ExternalStream(stream, device=device)):
+    # 0 is the default stream; an ExternalStream of 0 would be one of torch's own
+    s = t.cuda.ExternalStream(stream, device=device) if stream else t.cuda.default_stream(device)
+    with t.cuda.stream(s):
         return t.empty(nbytes, dtype=t.uint8, device=f"cuda:{device}")

@@ -100,3 +100,18 @@ def test_a_workspace_of_the_size_that_is_named():
     assert (out == 0).all()
     with pytest.raises(D.InvalidArgumentError, match="workspace"):
         D.q8_attend(c.cache, q, out, lens, max_len=length, workspace=ws[:need - 16])
+
+
+@pytest.mark.parametrize("other", ["default", "stream"])
+def test_the_workspace_belongs_to_the_calls_stream(other):
+    """A call on a stream that is not torch's current one: its workspace goes back to that stream's memory."""
+    target = torch.cuda.default_stream() if other == "default" else torch.cuda.Stream()
+    size = 48 << 20
+    with torch.cuda.stream(torch.cuda.Stream()):
+        ws = D.q8._scratch(0, size, target.cuda_stream)
+        at = ws.data_ptr()
+        del ws
+        mine = torch.empty(size, dtype=torch.uint8, device="cuda")
+        assert mine.data_ptr() != at
+    with torch.cuda.stream(target):
+        assert torch.empty(size, dtype=torch.uint8, device="cuda").data_ptr() == at
