@@ -114,8 +114,14 @@ def _ints(device: int, x, n: int, what: str) -> int:
 
 
 def _batch(device: int, n: int, tokens: int, max_q: int, q_start, slots, status) -> bytes:
+    _count(max_q, "max_q")
     return _BATCH.pack(n, tokens, max_q, _ints(device, q_start, n + 1, "q_start"), _ints(device, slots, n, "slots"),
                        0 if status is None else _ints(device, status, 1, "status"))
+
+
+def _count(x: int, what: str):
+    if not 0 <= x <= 0xFFFFFFFF:
+        _refuse(f"{what} must be 0 to 2^32 - 1, got {x}")
 
 
 def _rows(cache: Q8Cache, x, heads: int, what: str):
@@ -198,6 +204,7 @@ def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: 
             _refuse("masked must be on the cache's device with contiguous rows")
         mp, ms = masked.data_ptr(), masked.stride(0) if n > 1 else 0
     b = _batch(dev, n, tokens, max_q, q_start, slots, status)
+    _count(max_len, "max_len")
     if stream is None:
         stream = _stream_of(dev)
     wp, wn = None, 0
@@ -234,6 +241,8 @@ def workspace_bytes(cache: Q8Cache, tokens: int, heads: int, max_len: int = 0, *
     heads and this max_len runs, however the rows belong to sequences; with
     `n`, of a call without q_start whose n sequences have tokens / n rows each
     (defer_q8_attend_workspace; many rows a sequence need none)."""
+    for x, what in ((tokens, "tokens"), (heads, "heads"), (max_len, "max_len"), (n or 0, "n")):
+        _count(x, what)
     # the host only asks whether there is a q_start: with one, sequences may have any number of rows
     b = _BATCH.pack(1, tokens, 0, 1, 0, 0) if n is None else _BATCH.pack(n, tokens, 0, 0, 0, 0)
     return _workspace_bytes(cache, b, max_len, heads)

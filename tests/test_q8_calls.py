@@ -60,3 +60,14 @@ def test_workspace_bytes_serves_every_batch(dtype, hd, length):
                 assert need <= most and need == q8.workspace_bytes(c, tokens, 32, length, n=n)
         for max_q in (0, 1, 16, 64):
             assert q8._workspace_bytes(c, q8._batch(0, 3, tokens, max_q, ints(4), None, None), length, 32) <= most
+
+
+@pytest.mark.parametrize("bad", [-1, 1 << 32, (1 << 32) + 5])
+def test_counts_out_of_range_are_refused(bad):
+    c, kv, q = cache(), Array(4, 2, 64), Array(4, 4, 64)
+    for call in (lambda: D.q8_append(c, kv, kv, ints(4), max_q=bad), lambda: D.q8_attend(c, q, q, ints(4), max_q=bad),
+                 lambda: D.q8_attend(c, q, q, ints(4), max_len=bad), lambda: q8.workspace_bytes(c, bad, 4),
+                 lambda: q8.workspace_bytes(c, 4, bad), lambda: q8.workspace_bytes(c, 4, 4, bad),
+                 lambda: q8.workspace_bytes(c, 4, 4, n=bad)):
+        with pytest.raises(D.InvalidArgumentError, match="2\\^32"):
+            call()
