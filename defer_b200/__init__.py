@@ -350,10 +350,14 @@ class QuantKvCache:
         _check(_L().defer_qcache_download(self._h, slot, l, _f32p(k), _f32p(v)))
         return k[:n], v[:n]
 
-    def view(self, l: int) -> "_lib.Q8CacheC":
-        """One layer's device buffers (defer_q8_cache)."""
-        out = _lib.Q8CacheC()
+    def view(self, l: int) -> "q8.Q8LayerView":
+        """One layer's device buffers (defer_q8_cache), for q8_append, q8_read
+        and q8_attend: rows of it are float32. A call that writes them does not
+        change the lengths that this cache counts, and forward_q8 runs on the
+        model's own stream: wait for one before the other."""
+        out = q8.Q8LayerView()
         _check(_L().defer_qcache_view(self._h, l, ctypes.byref(out)))
+        out.owner = self
         return out
 
 

@@ -101,6 +101,33 @@ class Q8Cache:
         self._ref = ctypes.addressof(self._c)
 
 
+class Q8LayerView(_lib.Q8CacheC):
+    """One layer of a QuantKvCache (QuantKvCache.view), taken by q8_append,
+    q8_read and q8_attend like a Q8Cache; it keeps its QuantKvCache alive."""
+
+    owner = None
+    _cache = None
+
+
+def _cache_of(view) -> Q8Cache:
+    """The Q8Cache that a defer_q8_cache structure describes."""
+    if not isinstance(view, _lib.Q8CacheC):
+        _refuse(f"the cache must be a Q8Cache or a layer's view, got {type(view).__name__}")
+    c = getattr(view, "_cache", None)
+    if c is None:
+        t = sys.modules.get("torch")
+        if t is None:
+            _refuse("a layer's view needs torch arrays beside it")
+        c = Q8Cache.__new__(Q8Cache)
+        for name in ("k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail"):
+            setattr(c, name, None)
+        c.slots, c.kv_heads, c.cap, c.head_dim, c.device = view.slots, view.kv_heads, view.cap, view.head_dim, view.device
+        c.dtype = (t.float32, t.bfloat16, t.float16)[view.dtype]
+        c._c, c._ref = None, ctypes.addressof(view)
+        view._cache = c
+    return c
+
+
 def _ints(device: int, x, n: int, what: str) -> int:
     """Device pointer of an int32 array of n entries (None: NULL)."""
     if x is None:
@@ -142,6 +169,8 @@ def q8_append(cache: Q8Cache, k, v, pos, *, q_start=None, slots=None, max_q: int
     """Writes rows k, v [tokens, kv_heads, head_dim] at positions pos[i],
     pos[i] + 1, ... of each sequence i (defer_q8_append). pos, q_start, slots
     and status are int32 device arrays."""
+    if not isinstance(cache, Q8Cache):
+        cache = _cache_of(cache)
     dev, n = cache.device, pos.numel()
     kp, kt, kh = _rows(cache, k, cache.kv_heads, "k")
     vp, vt, vh = _rows(cache, v, cache.kv_heads, "v")
@@ -160,6 +189,8 @@ def q8_read(cache: Q8Cache, k_out, v_out, lens, *, start=None, slots=None, statu
     """Positions start[i] .. lens[i] - 1 of each sequence into k_out and v_out
     [n, kv_heads, rows, head_dim] (any strides of the first three); rows
     behind the last position are left as they were (defer_q8_read)."""
+    if not isinstance(cache, Q8Cache):
+        cache = _cache_of(cache)
     dev, n, shape = cache.device, lens.numel(), k_out.shape
     if len(shape) != 4 or shape[0] != n or shape[1] != cache.kv_heads or shape[3] != cache.head_dim:
         _refuse(f"k_out must be [{n}, {cache.kv_heads}, rows, {cache.head_dim}], got {tuple(shape)}")
@@ -189,6 +220,8 @@ def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: 
     head_dim ** -0.5. Long sequences need a workspace (a contiguous device
     array of workspace_bytes() bytes or more, used while the call runs): by
     default it is taken from torch's allocator on the call's stream."""
+    if not isinstance(cache, Q8Cache):
+        cache = _cache_of(cache)
     dev, n = cache.device, lens.numel()
     heads = q.shape[1] if len(q.shape) == 3 else 0
     qp, qt, qh = _rows(cache, q, heads, "q")
@@ -241,6 +274,8 @@ def workspace_bytes(cache: Q8Cache, tokens: int, heads: int, max_len: int = 0, *
     heads and this max_len runs, however the rows belong to sequences; with
     `n`, of a call without q_start whose n sequences have tokens / n rows each
     (defer_q8_attend_workspace; many rows a sequence need none)."""
+    if not isinstance(cache, Q8Cache):
+        cache = _cache_of(cache)
     for x, what in ((tokens, "tokens"), (heads, "heads"), (max_len, "max_len"), (n or 0, "n")):
         _count(x, what)
     # the host only asks whether there is a q_start: with one, sequences may have any number of rows

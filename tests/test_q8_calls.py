@@ -71,3 +71,11 @@ def test_counts_out_of_range_are_refused(bad):
                  lambda: q8.workspace_bytes(c, 4, 4, n=bad)):
         with pytest.raises(D.InvalidArgumentError, match="2\\^32"):
             call()
+
+
+def test_what_is_no_cache_is_refused():
+    q = Array(4, 4, 64)
+    for call in (lambda: D.q8_append(None, q, q, ints(4)), lambda: D.q8_attend(q, q, q, ints(4)),
+                 lambda: D.q8_read("layer", q, q, ints(4)), lambda: q8.workspace_bytes(object(), 4, 4)):
+        with pytest.raises(D.InvalidArgumentError, match="Q8Cache"):
+            call()
