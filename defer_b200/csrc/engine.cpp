@@ -931,11 +931,17 @@ void forward_q8(QuantCache* c, const uint32_t* slots, const uint32_t* tokens, si
     if (c->len[slots[i]] >= (size_t)c->cap) fail(kModel, "cache capacity " + std::to_string(c->cap) + " exceeded");
   }
   if (n == 0) return;
+  // a tensor-core step has 128 slots; more of them take several steps, to the same bits
+  const size_t most = m->tc_all ? std::min(n, (size_t)kTcM) : n;
   // the runner's own attention is not used: chunk partials of one chunk
-  if (!c->runner || c->runner->capacity() < (int)n) c->runner.reset(new Runner(m, (int)n, kAttnChunk));
-  c->runner->step_q8(*c, slots, tokens, (int)n);
-  if (logits_out)
-    for (size_t i = 0; i < n; i++) c->runner->download_logits((int)i, logits_out + i * m->cfg.vocab_size);
+  if (!c->runner || c->runner->capacity() < (int)most) c->runner.reset(new Runner(m, (int)most, kAttnChunk));
+  for (size_t at = 0; at < n; at += most) {
+    const size_t k = std::min(most, n - at);
+    c->runner->step_q8(*c, slots + at, tokens + at, (int)k);
+    if (logits_out)
+      for (size_t i = 0; i < k; i++)
+        c->runner->download_logits((int)i, logits_out + (at + i) * m->cfg.vocab_size);
+  }
 }
 
 // ----------------------------------------------------------- batch drivers

@@ -377,7 +377,8 @@ DEFER_API int defer_qcache_download(const defer_qcache* c, uint32_t slot, uint32
  * writes them does not change the slots' lengths that the handle counts. */
 DEFER_API int defer_qcache_view(const defer_qcache* c, uint32_t layer, defer_q8_cache* out);
 /* Model::forward (src/model.rs:376-520) of tokens[i] in slot slots[i], i < n,
- * all in one step: each slot's K and V rows are appended to the 8-bit cache
+ * all in one step (of a model whose token loops run on the tensor cores: in
+ * steps of 128 slots): each slot's K and V rows are appended to the 8-bit cache
  * and attention reads it; logits_out (NULL, or n * vocab_size floats) receives
  * the logits. No slot may be named twice. The projections are those of the
  * batched token loops; a slot's result does not depend on the other slots. */
