@@ -124,6 +124,7 @@ SIGNATURES = [
     ("defer_q8_attend", ctypes.c_int, [vp, ctypes.c_char_p, vp, u32, u32, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.c_int32,
                                        ctypes.c_float, vp, sz, vp]),
     ("defer_q8_attend_workspace", ctypes.c_int, [vp, ctypes.c_char_p, u32, u32, c_szp]),
+    ("defer_debug_q8_stall", ctypes.c_int, [ctypes.c_int32, u32]),
     ("defer_qcache_new", ctypes.c_int, [vp, u32, u32, ctypes.c_int32, ctypes.POINTER(vp)]),
     ("defer_qcache_free", None, [vp]),
     ("defer_qcache_len", sz, [vp, u32]),

@@ -707,6 +707,14 @@ int defer_debug_stall(defer_model* m, uint32_t wait_us) {
   });
 }
 
+int defer_debug_q8_stall(int32_t role, uint32_t wait_us) {
+  return guard([&] {
+    q8_check(role >= defer::kQ8StallQ && role <= defer::kQ8StallWeights, "role must be 1 to 5");
+    q8_check(wait_us >= 1 && wait_us <= 1000000u, "wait_us must be in 1..10^6");
+    defer::q8_stall_next(role, wait_us);
+  });
+}
+
 int defer_q8_append(const defer_q8_cache* cache, const defer_q8_batch* batch, const int32_t* pos, const void* k,
                     int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                     int64_t v_head_stride, void* stream) {

@@ -1174,6 +1174,18 @@ void attend_few(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream
 
 }  // namespace
 
+namespace {
+thread_local struct {
+  int role;
+  unsigned wait_us;
+} drill;
+}  // namespace
+
+void q8_stall_next(int role, unsigned wait_us) {
+  drill.role = role;
+  drill.wait_us = wait_us;
+}
+
 size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a) {
   if (!b.q_start && q8_tiles(c, b, a)) return 0;
   const int closed = a.max_len / kQ8Block * kQ8Block;
@@ -1194,7 +1206,14 @@ void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& args, cudaStre
   a.group = a.heads / c.kvh;
   a.group_inv = (unsigned)(0xFFFFFFFFull / (unsigned)a.group + 1);
   a.tiled = q8_tiles(c, b, a);
+  a.wait_ns = 2000000000ull;
+  a.stall = 0;
   if (a.tiled) {
+    if (drill.role) {
+      a.stall = drill.role;
+      a.wait_ns = drill.wait_us * 1000ull;
+      drill.role = 0;
+    }
     q8_attend_tiles(c, b, a, st);
     if (!b.q_start) return;  // every sequence has the same number of rows: none is left
   }

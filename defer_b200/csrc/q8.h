@@ -81,6 +81,8 @@ struct Q8Attend {
   int tiled;                   // sequences of more than kQ8FewRows rows are q8_attend_tiles'
   int group;                   // heads of a key head
   unsigned group_inv;          // 2^32 / group, rounded up
+  unsigned long long wait_ns;  // limit of the tile kernel's waits
+  int stall;                   // Q8Stall: an arrival of the tile kernel that is withheld (a drill), or 0
 };
 // Rows of a sequence and key head up to which the streaming kernel takes them
 // all: 4 passes over the cache with 16 rows each.
@@ -89,6 +91,12 @@ constexpr int kQ8FewRows = 64;
 // kernel's launch for them.
 bool q8_tiles(const Q8View& c, const Q8Batch& b, const Q8Attend& a);
 void q8_attend_tiles(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st);
+// A role of the tile kernel whose arrivals the drill withholds: the operands of
+// q, K or V, the scales, the weights.
+enum Q8Stall : int { kQ8StallQ = 1, kQ8StallK, kQ8StallV, kQ8StallScales, kQ8StallWeights };
+// The calling thread's next q8_attend that launches the tile kernel runs
+// with `role` stalled and every wait limited to wait_us.
+void q8_stall_next(int role, unsigned wait_us);
 size_t q8_attend_workspace(const Q8View& c, const Q8Batch& b, const Q8Attend& a);
 void q8_attend(const Q8View& c, const Q8Batch& b, const Q8Attend& a, cudaStream_t st);
 

@@ -55,13 +55,13 @@ namespace {
 constexpr int kQtM = 128;          // rows of a tile
 constexpr int kQtN = 128;          // positions of a block
 constexpr int kQtThreads = 17 * 32;
+constexpr unsigned long long kQtDrainNs = 2000000000ull;
 constexpr int kQtSlots = 4;        // ring of scales and masks
 // A weight's operand is 2^(x - m) s_V 2^(kQtUnit - D), where x + log2 s_V is at
 // most m + D + kQtLagD + 1: below 2^15.
 constexpr int kQtUnit = 10;
 constexpr float kQtLagD = 4.0f, kQtLagM = 16.0f;
 constexpr float kQtLeast = -100.0f;  // D of a row that has seen nothing; scale_exponent's least
-constexpr unsigned long long kQtWaitNs = 2000000000ull;
 
 // Scales and masks of one block of positions.
 struct QtScales {
@@ -71,6 +71,11 @@ struct QtScales {
   uint32_t show[kQtN / 32];     // bit per position: exists and is not hidden
 };
 
+// How long a wait of the CTA may take, and whether one has run out.
+struct QtLimit {
+  unsigned long long ns;
+  int failed;
+};
 template <int HDT>
 struct QtShared {
   unsigned char q[2][kQtM * HDT * 2];   // fp16 operands in core matrices
@@ -80,7 +85,7 @@ struct QtShared {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[kQtSlots];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
   uint32_t tmem;
-  int failed;
+  QtLimit limit;
   int open_odd;          // the open block's values hold a NaN or an infinity
   float red[2][2][4];
   int red_odd[2][4];
@@ -111,14 +116,14 @@ __device__ __forceinline__ bool qb_try(uint64_t* b, unsigned parity) {
 }
 // Bounded wait for the phase of `parity`; false when it ran out or another
 // role of the CTA has given up.
-__device__ __forceinline__ bool qb_wait(uint64_t* b, unsigned parity, int* failed) {
+__device__ __forceinline__ bool qb_wait(uint64_t* b, unsigned parity, QtLimit* limit) {
   if (qb_try(b, parity)) return true;
   const unsigned long long t0 = qt_time();
   for (unsigned spins = 1; !qb_try(b, parity); spins++) {
     if ((spins & 63u) == 0) {
-      if (*(volatile int*)failed) return false;
-      if (qt_time() - t0 > kQtWaitNs) {
-        *(volatile int*)failed = 1;
+      if (*(volatile int*)&limit->failed) return false;
+      if (qt_time() - t0 > limit->ns) {
+        *(volatile int*)&limit->failed = 1;
         return false;
       }
     }
@@ -272,7 +277,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     }
     for (int x = 0; x < kQtSlots; x++) qb_init(&S.sc_full[x], 128);
     qb_init(&S.drain, 1);
-    S.failed = 0;
+    S.limit.ns = a.wait_ns;
+    S.limit.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 16) {
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
   qt_after();
   const uint32_t tm = S.tmem;
   const uint32_t tm_s[2] = {tm, tm + 128}, tm_o[2] = {tm + 256, tm + 256 + HDT};
-  int* const failed = &S.failed;
+  QtLimit* const limit = &S.limit;
 
   const size_t sh = (size_t)s.slot * c.kvh + kvh;
   const int closed = len & ~(kQ8Block - 1);
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         }
         __syncwarp();
         qt_proxy();
-        qb_arrive(&S.q_full[wg]);
+        if (a.stall != kQ8StallQ) qb_arrive(&S.q_full[wg]);
       }
       const float fs = S.fac[wg * kQtM + row];
 
@@ -373,7 +379,7 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         const unsigned blk = n_sc + t;
         const QtScales& sc = S.sc[blk % kQtSlots];
         // the scores first: only then is the slot's phase the last one that was completed
-        ok = qb_wait(&S.s_full[wg], n_s & 1, failed) && qb_wait(&S.sc_full[blk % kQtSlots], (blk / kQtSlots) & 1, failed);
+        ok = qb_wait(&S.s_full[wg], n_s & 1, limit) && qb_wait(&S.sc_full[blk % kQtSlots], (blk / kQtSlots) & 1, limit);
         n_s++;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -480,10 +486,10 @@ __global__ void __launch_bounds__(kQtThreads, 1)
         }
         tm_wait_st();
         qt_before();
-        qb_arrive(&S.p_full[wg]);
+        if (a.stall != kQ8StallWeights) qb_arrive(&S.p_full[wg]);
       }
       n_sc += nb_all;
-      if (ok && nb) ok = __all_sync(0xffffffffu, qb_wait(&S.o_full[wg], n_q & 1, failed));
+      if (ok && nb) ok = __all_sync(0xffffffffu, qb_wait(&S.o_full[wg], n_q & 1, limit));
       if (nb) n_q++;
       T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)token * a.out.token + (int64_t)head * a.out.head;
       const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l), back = exp2i((int)D - kQtUnit);
@@ -612,12 +618,13 @@ __global__ void __launch_bounds__(kQtThreads, 1)
           *reinterpret_cast<uint4*>(d + 128) = make_uint4(o[4], o[5], o[6], o[7]);
         }
       if ((t + 1) * kQtN <= closed || t * kQtN >= len) return;
-      // the open block's tokens, over the zeros that the warps have put in their place
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + (int)is_v) : "memory");
+      // the open block's tokens, over the zeros that this warp has put in their
+      // place: no warp waits for another, which may have given up
+      __syncwarp();
 #pragma unroll 1
-      for (int u = ct; u < (len - closed) * (hd / 8); u += 128) {
+      for (int u = lane; u < (len - closed) * (hd / 8); u += 32) {
         const int p = closed + u / (hd / 8) - t * kQtN, d8 = u % (hd / 8);
-        if (p < 0 || p >= kQtN) continue;
+        if (p < 0 || p >= kQtN || ((p >> 3) & 3) != cw) continue;
         const T* y = tail + (u / (hd / 8)) * hd + d8 * 8;
         const bool hid = hide && hide[t * kQtN + p];
         uint32_t o[4];
@@ -662,16 +669,17 @@ __global__ void __launch_bounds__(kQtThreads, 1)
             sc.vs[ct] = vs;
             sc.lam[ct] = scale_exponent(vs);
           }
-          qb_arrive(&S.sc_full[n % kQtSlots]);
+          if (a.stall != kQ8StallScales) qb_arrive(&S.sc_full[n % kQtSlots]);
         }
-        if (n >= 2) ok = qb_wait(is_v ? &S.v_empty[st] : &S.k_empty[st], ph ^ 1, failed);
+        if (n >= 2) ok = qb_wait(is_v ? &S.v_empty[st] : &S.k_empty[st], ph ^ 1, limit);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         store(is_v ? S.v[st] : S.k[st], t);
         qt_proxy();
-        qb_arrive(is_v ? &S.v_full[st] : &S.k_full[st]);
+        // a drill withholds one warp's share: the others of the group go on
+        if (a.stall != (is_v ? kQ8StallV : kQ8StallK) || cw) qb_arrive(is_v ? &S.v_full[st] : &S.k_full[st]);
         if (t + 1 < nb) load(t + 1);
       }
     }
@@ -702,11 +710,11 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       const int nb[2] = {blocks_to(min(x0 + kQtM, x_end) - 1), x0 + kQtM < x_end ? blocks_to(x_end - 1) : 0};
       const int all = max(nb[0], nb[1]);
       for (int w = 0; w < 2 && ok; w++)
-        if (nb[w]) ok = qb_wait(&S.q_full[w], n_q[w]++ & 1, failed);
+        if (nb[w]) ok = qb_wait(&S.q_full[w], n_q[w]++ & 1, limit);
       if (!ok) break;
       qt_after();
       if (all) {
-        ok = qb_wait(&S.k_full[n & 1], (n >> 1) & 1, failed);
+        ok = qb_wait(&S.k_full[n & 1], (n >> 1) & 1, limit);
         if (!ok) break;
         qt_after();
         for (int w = 0; w < 2; w++)
@@ -715,11 +723,11 @@ __global__ void __launch_bounds__(kQtThreads, 1)
       }
       for (int t = 0; t < all && ok; t++) {
         const unsigned blk = n + t;
-        ok = qb_wait(&S.v_full[blk & 1], (blk >> 1) & 1, failed);
-        if (ok && t + 1 < all) ok = qb_wait(&S.k_full[(blk + 1) & 1], ((blk + 1) >> 1) & 1, failed);
+        ok = qb_wait(&S.v_full[blk & 1], (blk >> 1) & 1, limit);
+        if (ok && t + 1 < all) ok = qb_wait(&S.k_full[(blk + 1) & 1], ((blk + 1) >> 1) & 1, limit);
         for (int w = 0; w < 2 && ok; w++) {
           if (t >= nb[w]) continue;
-          ok = qb_wait(&S.p_full[w], n_p[w]++ & 1, failed);
+          ok = qb_wait(&S.p_full[w], n_p[w]++ & 1, limit);
           if (!ok) break;
           qt_after();
           values(w, blk, t > 0);
@@ -736,8 +744,8 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     qt_commit(&S.drain);
     const unsigned long long t0 = qt_time();
     while (!qb_try(&S.drain, 0))
-      if (qt_time() - t0 > kQtWaitNs) {
-        *(volatile int*)failed = 1;
+      if (qt_time() - t0 > kQtDrainNs) {  // not the drill's limit: what was issued has to end
+        limit->failed = 1;
         break;
       }
   }

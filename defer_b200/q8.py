@@ -258,6 +258,15 @@ def q8_attend(cache: Q8Cache, q, out, lens, *, q_start=None, slots=None, max_q: 
     return out
 
 
+def stall_next_attend(role: int, wait_us: int = 1000) -> None:
+    """Fault drill: this thread's next q8_attend of many 16-bit rows withholds
+    one role's arrivals with its bounded waits cut to wait_us
+    (defer_debug_q8_stall)."""
+    rc = _lib.load().defer_debug_q8_stall(role, wait_us)
+    if rc:
+        _check(rc)
+
+
 _LONG = 9000  # shorter sequences need no workspace, whatever the head size
 
 

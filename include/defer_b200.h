@@ -356,6 +356,13 @@ DEFER_API int defer_q8_attend(const defer_q8_cache* c, const defer_q8_batch* b, 
 DEFER_API int defer_q8_attend_workspace(const defer_q8_cache* c, const defer_q8_batch* b, uint32_t max_len,
                                         uint32_t heads, size_t* bytes);
 
+/* Fault drill (as defer_debug_stall): in the calling thread's next
+ * defer_q8_attend of many 16-bit rows one role of the kernel withholds its
+ * arrivals (1: q, 2: K, 3: V, 4: scales, 5: weights) and every bounded wait is
+ * limited to wait_us microseconds. The rows become NaN, bit 2 of the status word
+ * is set, nothing faults, and later calls are unaffected. */
+DEFER_API int defer_debug_q8_stall(int32_t role, uint32_t wait_us);
+
 /* A model's caches in 8 bits: `slots` sessions of up to `cap` positions (0:
  * max_position_embeddings; rounded up to 16), every layer, the open blocks in
  * fp32. For models whose head_dim is a multiple of 16 up to 256. */

@@ -79,3 +79,9 @@ def test_what_is_no_cache_is_refused():
                  lambda: D.q8_read("layer", q, q, ints(4)), lambda: q8.workspace_bytes(object(), 4, 4)):
         with pytest.raises(D.InvalidArgumentError, match="Q8Cache"):
             call()
+
+
+@pytest.mark.parametrize("role,wait_us", [(0, 1000), (6, 1000), (-1, 1000), (2, 0), (2, 10 ** 6 + 1)])
+def test_drill_refusals(role, wait_us):
+    with pytest.raises(D.InvalidArgumentError):
+        q8.stall_next_attend(role, wait_us)
