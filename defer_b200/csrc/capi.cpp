@@ -721,6 +721,8 @@ int defer_q8_append(const defer_q8_cache* cache, const defer_q8_batch* batch, co
   return guard([&] {
     const defer::Q8View c = q8_view(cache);
     const defer::Q8Batch b = q8_batch(c, batch);
+    // each sequence looks through the slots in front of its own: a kernel of minutes at 2^24 of them
+    q8_check(!b.slots || b.n <= 1 << 16, "an append names at most 2^16 slots");
     if (b.n == 0 || b.tokens == 0) return;
     need(pos, "pos");
     need(k, "k");

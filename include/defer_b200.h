@@ -319,7 +319,8 @@ typedef struct {
 /* Writes rows k and v [tokens][kv_heads][head_dim] of the cache's dtype
  * (strides of rows and heads in elements) at positions pos[i], pos[i] + 1, ...
  * of each sequence; pos [n] is device memory. The cache holds pos[i]
- * positions already, those of the open block in the tail. */
+ * positions already, those of the open block in the tail. With slots, at most
+ * 2^16 sequences (the kernel compares them with one another). */
 DEFER_API int defer_q8_append(const defer_q8_cache* c, const defer_q8_batch* b, const int32_t* pos, const void* k,
                               int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                               int64_t v_head_stride, void* stream);

@@ -85,3 +85,11 @@ def test_what_is_no_cache_is_refused():
 def test_drill_refusals(role, wait_us):
     with pytest.raises(D.InvalidArgumentError):
         q8.stall_next_attend(role, wait_us)
+
+
+def test_an_append_of_too_many_slots_is_refused():
+    """Its search for a slot that is named twice grows with the square of them."""
+    n = (1 << 16) + 1
+    c, kv = cache(slots=1 << 20, kvh=1, cap=16, hd=16), Array(n, 1, 16)
+    with pytest.raises(D.InvalidArgumentError, match="slots"):
+        D.q8_append(c, kv, kv, ints(n), slots=ints(n), stream=0)
