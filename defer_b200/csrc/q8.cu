@@ -258,8 +258,9 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // is (P . codes) * s_V with the scales outside the products, which run on the
 // tensor cores (mma m16n8k16, fp32 sums). The other operand is made as exact
 // as the cache's type asks: a q row is scaled by a power of two so that its
-// largest element is in [2^14, 2^15) and held as one fp16 term (bf16 and fp16
-// rows: no bit lost) or two (fp32: 22 bits). The weights of a block are taken
+// largest element is in [2^14, 2^15) and held as one fp16 term (a bf16 or fp16
+// row: its own bits, down to elements 2^31 below the row's largest) or two
+// (fp32: 22 bits; a third term changes no error that was measured). The weights of a block are taken
 // relative to the block's own largest score, P = 2^(x - max_block x) (x: score
 // in base 2), times 2^14 in two fp16 terms: 22 bits, with one term (11 bits)
 // the errors of 16-bit results are more than their own rounding. The block's
@@ -289,15 +290,16 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // open block (fp32 or 16-bit tokens) is added at the end by the last split, in
 // fp32.
 //
-// What bounds it: the issue of instructions, not the bytes. A step of 16
-// positions and 128 dims costs a warp about 370 instructions (112 of them turn
-// codes into fp16), a CTA's start, merges and open block about 5 us beside its
-// steps of 0.9 us. 8 sessions of 4096 positions (8B heads, fp32): 27 us, 2.5
-// TB/s; one sequence of 131077 (bf16): 62 us, 4.3 TB/s; 512 sessions of 16 to
-// 767 (135M heads): 37 us, 2.3 TB/s. CTAs of 4 warps let 4 of them overlap on
-// an SM: with 8 warps the last one took 43 us, 127 short sequences 78 instead
-// of 49. A ring of asynchronous copies in shared memory in place of the direct
-// loads: 53 us.
+// What bounds it: waiting. Of 64 sequences (bf16) an SM issues 1.3 of 4
+// instructions a cycle with 20 % of its warps active; the largest stalls are
+// the loads (2.5 cycles an instruction) and the cluster's last CTA (2.3). A
+// CTA's start, merges and open block take about 5 us beside its steps of 16
+// positions and 128 dims. 8 sessions of 4096 positions (8B heads, fp32): 27 us,
+// 2.5 TB/s; one sequence of 131077 (bf16): 68 us, 4.0 TB/s; 64 sequences of 129
+// to 8191 (bf16): 159 us, 3.5 TB/s; 512 sessions of 16 to 767 (135M heads): 39
+// us, 2.2 TB/s. CTAs of 4 warps let 4 of them overlap on an SM: with 8 warps
+// (both with cold caches) the 64 sequences take 213 us instead of 164, 127
+// sequences of 128 positions 88 instead of 59.
 constexpr int kQsWarps = 4;
 constexpr int kQsCluster = 8;     // splits of a cluster
 constexpr int kQsMaxSplits = 64;  // of a sequence
@@ -326,12 +328,12 @@ constexpr size_t qs_smem() {
 
 // Splits of a sequence of `rows` rows a key head with `closed` positions in
 // closed blocks. Up to 16 rows: of 4 units or more (a single short sequence is
-// a matter of latency: 14 us instead of 16 for 1041 positions of the 135M
-// heads), up to the 8 that one cluster merges; of 16 units or more when that
-// makes more of them (a CTA's start and its merges cost about 5 units: 64
-// sequences of up to 8191 positions take 150 us, 175 with 8 units). More rows
-// are many CTAs anyway: of 8 units or more (512 rows over 2048 positions of the
-// 135M heads: 43 us instead of 65).
+// a matter of latency: with cold caches 16 us, 18 with 8 units, for 1041
+// positions of the 135M heads), up to the 8 that one cluster merges; of 16 units
+// or more when that makes more of them (a CTA's start and its merges cost about
+// 5 units: 64 sequences of up to 8191 positions take 164 us, 187 with 8 units).
+// More rows are many CTAs anyway: of 8 units or more (512 rows over 2048
+// positions of the 135M heads: 60 us, 68 with 4 units).
 template <int HDP>
 __host__ __device__ __forceinline__ int qs_splits(int closed, int64_t rows) {
   const int units = (closed + QsShape<HDP>::UNIT - 1) / QsShape<HDP>::UNIT;

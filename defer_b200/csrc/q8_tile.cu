@@ -18,7 +18,9 @@
 // no bit by that; of a bf16 token, an element 2^32 times smaller than the
 // block's largest begins to (fp16 numbers end at 2^-24), as does an element of
 // a bf16 q row 2^31 times smaller than the row's largest. Weights are two fp16
-// terms (22 bits). Output and sums stay in fp32 (tensor memory, registers).
+// terms (22 bits). Output and sums stay in fp32 (tensor memory, registers): the
+// chain of 512 sums over 4096 positions may be some 2^-16 off, 2^-7 of a bf16
+// result's rounding, 2^-4 of an fp16 one's.
 //
 // Work: a CTA takes two tiles of 128 rows (rows of the heads that share a key
 // head, token after token), so that a converted block of 128 positions feeds
@@ -31,12 +33,14 @@
 // they came from and are the A operand from there. The order of the products
 // (PV of tile 0, scores of tile 0 of the next block, the same of tile 1) keeps
 // every buffer's reuse behind its last reader without a wait of its own.
-// What bounds it: the way of a tile from its scores over the softmax (2.3 us)
-// to its products and back, with the other tile's products in between: a block
-// of 128 positions takes about 3.3 us for two tiles, of which the products are
-// 1.1 at full rate and the exponentials as much. Four prompt pieces of 170 to
-// 512 rows over 1024 to 4096 positions (8B heads, bf16): 194 us, 399 TFLOP/s;
-// with the converting warps shared by K and V 230 us, one tile a CTA 277 us.
+// What bounds it: the way of a tile from its scores over the softmax to its
+// products and back, with the other tile's products in between: a block of 128
+// positions takes about 4.7 us for two tiles, of which the products are 2.2 at
+// full rate (three products' worth: the weights have two terms). Four prompt
+// pieces of 170 to 512 rows over 1024 to 4096 positions (8B heads, bf16): 278
+// us, 279 TFLOP/s without the second term's products. With one term of the
+// weights it was 194 us; then, converting warps shared by K and V took 230, one
+// tile a CTA 277.
 // Every wait is bounded: one that runs out fills the rows with NaN, sets
 // kQ8Timeout in the status word and lets the CTA free its tensor memory.
 #include <cuda_runtime.h>

@@ -303,7 +303,9 @@ typedef struct {
  * each; rows behind q_start[n] are left as they were) and lives in slot
  * slots[i] (NULL: slot i; negative: the sequence is skipped and its rows are
  * left as they were). max_q: the largest number of rows of a sequence (0:
- * tokens); it sizes the launch and changes no result of defer_q8_append.
+ * tokens). It sizes the launch: sequences of more rows are still taken as a
+ * whole, with the same result of defer_q8_append and, of defer_q8_attend, one
+ * whose sums may be taken in another order.
  * q_start, slots and status are device memory. A sequence whose slot, rows,
  * position or length is out of range is skipped (defer_q8_attend fills its
  * rows with NaN where the rows themselves are valid), as is, when appending,
@@ -340,11 +342,16 @@ DEFER_API int defer_q8_read(const defer_q8_cache* c, uint32_t n, const int32_t* 
  * lens[i]. masked (NULL, or device bytes [n] with row stride mask_stride, 0 or
  * at least cap): position t of sequence i is hidden where masked[i *
  * mask_stride + t] is not 0. out = sum_t p_t V_t, p = softmax(scale * q . K_t)
- * over the positions seen, 0 when there are none; softmax and sums in fp32.
- * max_len: the longest length (0: cap); it sizes the launch, and a sequence
- * that is longer is still attended as a whole. A sequence's
- * result depends on its own rows, length and cache only, not on the call's
- * other sequences. */
+ * over the positions seen, 0 when there are none; softmax and sums in fp32, the
+ * weights rounded to 22 bits for the products with the values. Scores are sums
+ * of products with q (of fp32 rows: 22 bits of each element). For more than 64
+ * rows a key head of a 16-bit cache with head_dim up to 128, values that are
+ * 2^20 times smaller than another visible block's count with 15 bits, 2^30
+ * times smaller with 5. max_len: the longest length (0: cap). It sizes the
+ * launch: a sequence that is longer is still attended as a whole, its sums taken
+ * in another order. With max_q and max_len as they are or larger (or 0), a
+ * sequence's result depends on its own rows, length and cache only, not on the
+ * call's other sequences. */
 DEFER_API int defer_q8_attend(const defer_q8_cache* c, const defer_q8_batch* b, const int32_t* lens,
                               uint32_t max_len, uint32_t heads, const void* q, int64_t q_token_stride,
                               int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
