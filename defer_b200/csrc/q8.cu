@@ -260,11 +260,11 @@ __global__ void __launch_bounds__(128) k_q8_read(Q8View c, int n, const int* __r
 // as the cache's type asks: a q row is scaled by a power of two so that its
 // largest element is in [2^14, 2^15) and held as one fp16 term (a bf16 or fp16
 // row: its own bits, down to elements 2^31 below the row's largest) or two
-// (fp32: 22 bits; a third term changes no error that was measured). The weights of a block are taken
-// relative to the block's own largest score, P = 2^(x - max_block x) (x: score
-// in base 2), times 2^14 in two fp16 terms: 22 bits, with one term (11 bits)
-// the errors of 16-bit results are more than their own rounding. The block's
-// products P . codes come out of the tensor core by themselves and are added to
+// (fp32: 22 bits; a third term changes no error that was measured). The weights
+// of a block are taken relative to the block's own largest score, P = 2^(x -
+// max_block x) (x: score in base 2), times 2^14 in two fp16 terms: 22 bits, with
+// one term (11 bits) the errors of 16-bit results are more than their own
+// rounding; a weight 2^39 below the block's largest ends. The block's products P . codes come out of the tensor core by themselves and are added to
 // fp32 registers times 2^(max_block x - m) s_V, m the running maximum of the
 // scores: no block's values, however large, cost the others bits, and nothing
 // is summed in a long chain inside the tensor core. The sum of the weights is
