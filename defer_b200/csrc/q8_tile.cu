@@ -13,12 +13,13 @@
 // takes bits from it. A weight ends at 2^-25, 2^-35 of the row's largest weight
 // times value scale: where one block's values are 2^20 times the others', those
 // keep 15 bits, where they are 2^30 times, 5. The tokens of the open
-// block are 16-bit numbers: scaled by a power of two for the block, its largest
-// element to 2^15 or more, they are fp16 operands like codes. fp16 tokens lose
-// no bit by that; of a bf16 token, an element 2^32 times smaller than the
-// block's largest begins to (fp16 numbers end at 2^-24), as does an element of
-// a bf16 q row 2^31 times smaller than the row's largest. Weights are two fp16
-// terms (22 bits). Output and sums stay in fp32 (tensor memory, registers): the
+// block are 16-bit numbers: scaled by a power of two for the block they are fp16
+// operands like codes, values with their largest at 2^6, like a code, or as far
+// up as 2^15 where their smallest need it. fp16 tokens lose no bit by that; of a
+// bf16 token, an element 2^32 times smaller than the block's largest begins to
+// (fp16 numbers end at 2^-24), as does an element of a bf16 q row 2^31 times
+// smaller than the row's largest. At 2^15 the block's weights end 2^9 earlier
+// than other blocks'. Weights are two fp16 terms (22 bits). Output and sums stay in fp32 (tensor memory, registers): the
 // chain of 512 sums over 4096 positions may be some 2^-16 off, 2^-7 of a bf16
 // result's rounding, 2^-4 of an fp16 one's.
 //
@@ -91,7 +92,7 @@ struct QtShared {
   uint32_t tmem;
   QtLimit limit;
   int open_odd;          // the open block's values hold a NaN or an infinity
-  float red[2][2][4];
+  float red[2][3][4];
   int red_odd[2][4];
   float fac[2 * kQtM];   // row factors
 };
@@ -560,32 +561,43 @@ __global__ void __launch_bounds__(kQtThreads, 1)
     const float* ksc = c.ks + sh * (c.cap / kQ8Block);
     const float* vsc = c.vs + sh * (c.cap / kQ8Block);
     float open_k, open_v;
-    {  // the open block's power-of-two scales: its largest finite element that is not hidden becomes [2^15, 2^16)
-      float ak = 0.0f, av = 0.0f;
+    {
+      // The open block's power-of-two scales, from its finite elements that are
+      // not hidden. Keys: the largest becomes [2^15, 2^16). Values: the largest
+      // becomes [2^6, 2^7), as a code, so that the block's weights end where
+      // other blocks' do; or as far up as [2^15, 2^16) when the last bits of the
+      // smallest would else be below fp16's 2^-24.
+      float ak = 0.0f, av = 0.0f, nv = FLT_MAX;
       bool odd = false;
       for (int x = ct; x < (len - closed) * hd; x += 128) {
         if (hide && hide[closed + x / hd]) continue;
         const float yk = fabsf(E::to(kt[x])), yv = fabsf(E::to(vt[x]));
         ak = fmaxf(ak, yk <= FLT_MAX ? yk : 0.0f);
         av = fmaxf(av, yv <= FLT_MAX ? yv : 0.0f);
+        nv = fminf(nv, yv > 0.0f ? yv : FLT_MAX);
         odd |= !(yv <= FLT_MAX);
       }
       ak = warp_max_all(ak);
       av = warp_max_all(av);
+      nv = -warp_max_all(-nv);
       odd = __any_sync(0xffffffffu, odd);
       if (lane == 0) {
         S.red[is_v][0][cw] = ak;
         S.red[is_v][1][cw] = av;
+        S.red[is_v][2][cw] = nv;
         S.red_odd[is_v][cw] = odd;
       }
       asm volatile("bar.sync %0, 128;" ::"r"(1 + (int)is_v) : "memory");
       const float* rk = S.red[is_v][0];
       const float* rv = S.red[is_v][1];
+      const float* rn = S.red[is_v][2];
       const float mk = fmaxf(fmaxf(rk[0], rk[1]), fmaxf(rk[2], rk[3]));
       const float mv = fmaxf(fmaxf(rv[0], rv[1]), fmaxf(rv[2], rv[3]));
+      const int least = exponent_of(fminf(fminf(rn[0], rn[1]), fminf(rn[2], rn[3])));
+      const int top = max(exponent_of(mv), -96), last = TYPE == kQ8F16 ? max(least - 10, -24) : least - 7;
       // exponents from -96: smaller blocks keep fewer than their own bits
       open_k = mk > 0.0f ? exp2i(max(exponent_of(mk), -96) - 15) : 1.0f;
-      open_v = mv > 0.0f ? exp2i(max(exponent_of(mv), -96) - 15) : 1.0f;
+      open_v = mv > 0.0f ? exp2i(top - min(max(top - last - 24, 6), 15)) : 1.0f;
       const int* ro = S.red_odd[is_v];
       if (ct == 0 && !is_v) S.open_odd = ro[0] | ro[1] | ro[2] | ro[3];
     }

@@ -17,14 +17,24 @@ def on_tiles(dtype, hd, rows, group):
     return dtype != F32 and hd <= 128 and rows * group > 64
 
 
-def steps(c, slot):
+def steps(c, slot, hidden=None):
     """What the value codes of a slot's positions count in, [kvh, len]: the
-    block's scale; in the open block 2^-15 of its largest value."""
+    block's scale; in the open block 2^-6 of its largest visible value, or as
+    little as 2^-15 of it where its smallest ones need that to keep their bits
+    above 2^-24."""
     p = c.plain[slot][1]
     s = p.closed()[1].astype(float).repeat(BLOCK, 1)
     x = np.abs(p.x[s.shape[1]:].astype(float))  # [open positions, kvh, hd]
-    a = x.max((0, 2), initial=0.0, where=np.isfinite(x))
-    return np.concatenate([s, np.repeat(a[:, None] * 2.0 ** -15, len(x), 1)], 1)
+    if hidden is not None:
+        x = np.where(np.asarray(hidden, bool)[s.shape[1]:len(p.x), None, None], 0.0, x)
+    x = np.where(np.isfinite(x), x, 0.0)
+    top = x.max((0, 2), initial=0.0)
+    low = np.where(x > 0, x, np.inf).min((0, 2), initial=np.inf)
+    with np.errstate(all="ignore"):
+        e, f = np.floor(np.log2(top)), np.floor(np.log2(low))
+        last = np.maximum(f - 10, -24) if c.dtype == F16 else f - 7
+        z = np.where(top > 0, np.exp2(e - np.clip(e - last - 24, 6, 15)), 1.0)
+    return np.concatenate([s, np.repeat(z[:, None], len(x), 1)], 1)
 
 
 def check(c, slots, rows, heads, q=None, hidden=None, scale=None, causal=True, **kw):
@@ -44,7 +54,7 @@ def check(c, slots, rows, heads, q=None, hidden=None, scale=None, causal=True, *
         k, v = c.values(s)
         seen = [lens[i] - (rows - 1 - j) if causal else lens[i] for j in range(rows)]
         e = Exact(q[i * rows:(i + 1) * rows].double().cpu().numpy(), k, v, seen,
-                  None if hidden is None else hidden[i], sc, steps(c, s))
+                  None if hidden is None else hidden[i], sc, steps(c, s, None if hidden is None else hidden[i]))
         w = e.worst(out[i * rows:(i + 1) * rows], c.dtype, on_tiles(c.dtype, c.hd, rows, heads // c.kvh))
         assert w <= 1, (i, s, lens[i], w)
     return out
@@ -131,3 +141,15 @@ def test_keys_near_the_largest_number(dtype, rows, at):
         step = torch.finfo(dtype).eps
         bad = ((out - want).abs() > step * want.abs()) | torch.isnan(out)
         assert bad.sum().item() == 0, (size, out[0, 0, :4].tolist(), want[:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_an_ordinary_open_block_beside_large_values(dtype, hd):
+    """Tiles: a closed block's value 2^13 times the others leaves the open block's weights their bits."""
+    c = Case(1, 1, 64, hd, "int8", dtype, seed=13)
+    k, v = c.randn(47, 1, hd), c.randn(47, 1, hd)
+    v[:32] = 0
+    v[5, 0, 3] = 2.0 ** 13
+    c.append([0], [47], k, v)
+    check(c, [0], 140, 4, causal=False)
